@@ -229,6 +229,52 @@ int ovc_attention_ex(const void* q8, const void* k8, const void* v_packed, const
                      int64_t repair_rows, void* out, float* lse, int flags, int64_t B, int64_t Sq, int64_t Sk,
                      int64_t H, float softmax_scale, int mid_window_blocks, uint32_t* status, void* stream);
 
+/* ---- Rotary positions with several axes, with the RMS norm of the query and key heads ----
+ *
+ * No counterpart in the reference, whose callers rotate Q and K before they call it.
+ *   y = turn(x * w / sqrt(mean(x^2) + eps)); each pair (a, b) of a head's channels becomes
+ *   (a cos t - b sin t, a sin t + b cos t), t = 2 pi * turns[pair] * positions[token][pair_axis[pair]],
+ * computed in float32 (t in float64) and rounded once.  Pair p is the channels (2p, 2p + 1), or with half_split
+ * (p, p + 64); turns[p] = 0 leaves a pair unturned.  A null weight means no norm for that tensor.
+ */
+#define OVC_POSITIONS_I32 0
+#define OVC_POSITIONS_I64 1
+#define OVC_POSITIONS_F32 2
+
+typedef struct ovc_rotary {
+    const void* positions;          /* device: [S, axes], or [B, S, axes] with position_batch_stride = S * axes */
+    int64_t position_batch_stride;  /* in elements; 0: every batch item has the same positions */
+    const double* turns;            /* HOST: 64 frequencies in turns per position (read during the call) */
+    const uint8_t* pair_axis;       /* HOST: 64 axis indices < axes (read during the call) */
+    const float* q_weight;          /* device: [128] or null */
+    const float* k_weight;          /* device: [128] or null */
+    int position_type;              /* OVC_POSITIONS_* */
+    int axes;                       /* 1 .. 64 */
+    int half_split;
+    float eps;
+} ovc_rotary;
+
+/*
+ * Rotated (and normalised) Q and K in their own 16-bit type.
+ *   q [B,S,Hq,128], k [B,S,Hk,128]: strides[3] = elements from one batch item, token and head to the next, multiples
+ *   of 8 (a slice of a fused projection is read in place); q_out, k_out dense, not overlapping q or k.
+ */
+int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype, int64_t B,
+                  int64_t S, int64_t Hq, int64_t Hk, const ovc_rotary* rotary, void* q_out, void* k_out, void* stream);
+
+/*
+ * ovc_quantize_per_block of rotated (and normalised) Q and K, both in one launch.  The rotated values are not rounded
+ * to 16 bits in between.  q, k dense [B,S,H,128].
+ */
+int ovc_quantize_qk_rotary(const void* q, const void* k, int dtype, int64_t B, int64_t S, int64_t H,
+                           const ovc_rotary* rotary, void* q8, void* k8, float* q_descale, int64_t q_descale_stride,
+                           float* k_descale, int64_t k_descale_stride, void* stream);
+
+/* ovc_prepare_fused with rotated (and normalised) Q and K. */
+int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H,
+                             const ovc_rotary* rotary, void* q8, void* k8, void* v_packed, float* q_descale,
+                             float* k_descale, float* v_descale, float* amax_ws, void* stream);
+
 /* ---- VC-Attention baseline: V-Smooth preparation and the mean-restoring attention variant ----
  *
  * Replaces the Triton kernels and launches of src/open_vc_attn/_kernels/blackwell/v_smooth.py and the

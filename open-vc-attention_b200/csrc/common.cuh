@@ -20,6 +20,11 @@ inline int check_launch() {
     return OVC_OK;
 }
 
+// The V part of the fused preparation (prep.cu): per-head max |v| into amax_ws (which an earlier kernel on the stream has
+// reset), then the cast with the packed layout.  Arguments are the callers' to check.
+int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, float* amax_ws, void* v_packed, float* v_descale,
+                            void* stream);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int kTile = 128;  // tokens per quantisation block and per key tile

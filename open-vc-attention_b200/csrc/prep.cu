@@ -11,13 +11,10 @@
 // scale decides the code.  Every global access is a 16-byte (or 8-byte for FP8 rows) vector
 // access covering whole 128-byte lines per warp.
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include <atomic>
 
 #include "common.cuh"
+#include "rows.cuh"
 
 namespace ovc {
 
@@ -26,70 +23,12 @@ void set_last_cuda_error(int code) { g_last_cuda_error = code; }
 
 namespace {
 
-constexpr float kQMax = 448.0f;
-constexpr float kFloor = 1e-12f;
-
-__device__ __forceinline__ uint4 ld_stream(const void* p) {
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
-    return r;
-}
-
-// Eight 16-bit floats (one uint4) widened exactly to float32.
-template <int DT>
-__device__ __forceinline__ void widen8(const uint4& raw, float (&f)[8]) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (DT == OVC_BF16) {
-            f[2 * i] = __uint_as_float(w[i] << 16);
-            f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-        } else {
-            const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-            f[2 * i] = p.x;
-            f[2 * i + 1] = p.y;
-        }
-    }
-}
-
-__device__ __forceinline__ float absmax8(const float (&f)[8], float m) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
-    return m;
-}
-
-__device__ __forceinline__ float clamp448(float x) { return fminf(fmaxf(x, -kQMax), kQMax); }
-
-// Four float32 -> four E4M3 bytes (a in the lowest byte), RNE.
-__device__ __forceinline__ uint32_t cast4(float a, float b, float c, float d) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
-}
-
-__device__ __forceinline__ uint2 quantize8(const float (&f)[8], float scale) {
-    uint2 out;
-    out.x = cast4(clamp448(__fmul_rn(f[0], scale)), clamp448(__fmul_rn(f[1], scale)),
-                  clamp448(__fmul_rn(f[2], scale)), clamp448(__fmul_rn(f[3], scale)));
-    out.y = cast4(clamp448(__fmul_rn(f[4], scale)), clamp448(__fmul_rn(f[5], scale)),
-                  clamp448(__fmul_rn(f[6], scale)), clamp448(__fmul_rn(f[7], scale)));
-    return out;
-}
-
 __device__ __forceinline__ float4 decode4(uint32_t codes) {
     const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes & 0xFFFFu), __NV_E4M3);
     const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes >> 16), __NV_E4M3);
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     return make_float4(a.x, a.y, b.x, b.y);
-}
-
-__device__ __forceinline__ float warp_max(float m) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    return m;
 }
 
 // Max over the 128 threads of a CTA; every thread gets the result.
@@ -109,16 +48,6 @@ struct BlockQuantArgs {
     int sources;       // 1 or 2 tensors quantised by one launch
     float* amax_init;  // optional [H]: reset to 0 by the (block 0, source 0) CTAs
 };
-
-// Max over the 256 threads of a CTA; every thread gets the result.  `part` is caller-provided shared
-// memory (8 floats) so that consecutive reductions can alternate between two buffers.
-__device__ __forceinline__ float cta256_max(float m, float* part) {
-    m = warp_max(m);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
-    __syncthreads();
-    return fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])),
-                 fmaxf(fmaxf(part[4], part[5]), fmaxf(part[6], part[7])));
-}
 
 constexpr int kBlocksPerCta = 4;  // consecutive 128-token blocks handled by one CTA of the Q/K quantiser
 
@@ -453,6 +382,26 @@ int static_amax_pointer(float** out) {
 
 }  // namespace
 
+namespace ovc {
+
+int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, float* amax_ws, void* v_packed, float* v_descale,
+                            void* stream) {
+    const int64_t blocks = ceil_div(S, kTile), S_pad = blocks * kTile;
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(H), 1);
+    const int h = static_cast<int>(H);
+    auto s = static_cast<cudaStream_t>(stream);
+    if (dtype == OVC_BF16) {
+        head_amax_kernel<OVC_BF16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
+        cast_pack_kernel<OVC_BF16><<<grid, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
+    } else {
+        head_amax_kernel<OVC_F16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
+        cast_pack_kernel<OVC_F16><<<grid, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
+    }
+    return check_launch();
+}
+
+}  // namespace ovc
+
 extern "C" {
 
 int ovc_version(void) { return 1; }
@@ -521,7 +470,6 @@ int ovc_prepare_fused(const void* q, const void* k, const void* v, int dtype, in
         return OVC_ERR_ARGUMENT;
     const int64_t blocks = ceil_div(S, kTile);
     const int64_t q_blocks = (blocks + 1) / 2 * 2;
-    const int64_t S_pad = blocks * kTile;
     auto s = static_cast<cudaStream_t>(stream);
     const int h = static_cast<int>(H);
     BlockQuantArgs a{};
@@ -531,17 +479,9 @@ int ovc_prepare_fused(const void* q, const void* k, const void* v, int dtype, in
     a.descale_stride[0] = q_blocks, a.descale_stride[1] = blocks;
     a.sources = 2, a.amax_init = amax_ws;
     const dim3 grid_qk(static_cast<unsigned>(ceil_div(blocks, kBlocksPerCta)), static_cast<unsigned>(H), 2);
-    const dim3 grid_v(static_cast<unsigned>(blocks), static_cast<unsigned>(H), 1);
-    if (dtype == OVC_BF16) {
-        quant_block_kernel<OVC_BF16><<<grid_qk, 256, 0, s>>>(a, S, h, static_cast<int>(blocks));
-        head_amax_kernel<OVC_BF16><<<grid_v, 128, 0, s>>>(v, amax_ws, S, h);
-        cast_pack_kernel<OVC_BF16><<<grid_v, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
-    } else {
-        quant_block_kernel<OVC_F16><<<grid_qk, 256, 0, s>>>(a, S, h, static_cast<int>(blocks));
-        head_amax_kernel<OVC_F16><<<grid_v, 128, 0, s>>>(v, amax_ws, S, h);
-        cast_pack_kernel<OVC_F16><<<grid_v, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
-    }
-    return check_launch();
+    if (dtype == OVC_BF16) quant_block_kernel<OVC_BF16><<<grid_qk, 256, 0, s>>>(a, S, h, static_cast<int>(blocks));
+    else quant_block_kernel<OVC_F16><<<grid_qk, 256, 0, s>>>(a, S, h, static_cast<int>(blocks));
+    return launch_amax_cast_pack_v(v, dtype, S, H, amax_ws, v_packed, v_descale, stream);
 }
 
 int ovc_pack_v(const void* codes, int64_t B, int64_t S, int64_t H, void* packed, void* stream) {

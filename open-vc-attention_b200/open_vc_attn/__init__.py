@@ -49,6 +49,24 @@ def raw_forward(*args, **kwargs):
     return implementation(*args, **kwargs)
 
 
+def rotary_plan(*args, **kwargs):
+    from .rotary import rotary_plan as implementation
+
+    return implementation(*args, **kwargs)
+
+
+def grid_positions(*args, **kwargs):
+    from .rotary import grid_positions as implementation
+
+    return implementation(*args, **kwargs)
+
+
+def rotary_qk(*args, **kwargs):
+    from .rotary import rotary_qk as implementation
+
+    return implementation(*args, **kwargs)
+
+
 __all__ = [
     "attention",
     "attention_fp8",
@@ -57,4 +75,7 @@ __all__ = [
     "prepare_v_repair",
     "attention_v_repair",
     "raw_forward",
+    "rotary_plan",
+    "grid_positions",
+    "rotary_qk",
 ]

@@ -16,6 +16,16 @@ STATUS_WAIT_EXPIRED = 1
 
 _p, _i, _l, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
 
+
+class OvcRotary(ctypes.Structure):
+    """struct ovc_rotary of include/ovc.h."""
+
+    _fields_ = [
+        ("positions", _p), ("position_batch_stride", _l), ("turns", _p), ("pair_axis", _p), ("q_weight", _p), ("k_weight", _p),
+        ("position_type", _i), ("axes", _i), ("half_split", _i), ("eps", _f),
+    ]
+
+
 SIGNATURES = {
     "ovc_version": (_i, []),
     "ovc_error_string": (ctypes.c_char_p, [_i]),
@@ -34,6 +44,9 @@ SIGNATURES = {
     "ovc_selftest_wait": (_i, [_p, _l, _p, _p]),
     "ovc_copy_head_slice": (_i, [_p, _l, _l, _p, _l, _l, _l, _l, _l, _i, _p]),
     "ovc_attention_ex": (_i, [_p, _p, _p, _p, _l, _p, _p, _p, _l, _p, _p, _i, _l, _l, _l, _l, _f, _i, _p, _p]),
+    "ovc_rotary_qk": (_i, [_p, _p, _p, _p, _i, _l, _l, _l, _l, _p, _p, _p, _p]),
+    "ovc_quantize_qk_rotary": (_i, [_p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _l, _p, _l, _p]),
+    "ovc_prepare_fused_rotary": (_i, [_p, _p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "ovc_vs_assign": (_i, [_p, _p, _p, _l, _l, _l, _p]),
     "ovc_vs_accumulate": (_i, [_p, _p, _p, _p, _l, _l, _l, _p]),
     "ovc_vs_update_centers": (_i, [_p, _p, _p, _l, _l, _p]),

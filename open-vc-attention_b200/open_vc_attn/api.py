@@ -98,33 +98,47 @@ def _fused_preparation_eligible(q, k, v, *, version, mode, causal, return_lse):
     )
 
 
-def prepare_fp8(q, k, v):
+def _check_rotary(rotary, q, k):
+    from .rotary import RotaryPlan
+
+    RotaryPlan.check(rotary, q, k)
+
+
+def prepare_fp8(q, k, v, *, rotary=None):
     """Q/K: per 128 tokens per head; V: per sequence per head; E4M3 max 448.
 
     The returned tensors retain descales in FP32.  Preparation is stream ordered.
+    ``rotary`` (from ``rotary_plan``): Q and K are normalised and rotated on the way, without a rounding to 16 bits.
     """
     validate_qkv(q, k, v)
+    if rotary is not None:
+        _check_rotary(rotary, q, k)
     from .quantization import fp8_quantize_per_block, fp8_quantize_per_head
 
     with torch.cuda.device(q.device):
         q, k, v, layout, shape = _layout(q, k, v)
-        q8, qs = fp8_quantize_per_block(q, block_l=128)
-        k8, ks = fp8_quantize_per_block(k, block_l=128)
+        if rotary is not None:
+            from .rotary import quantize_qk
+
+            q8, qs, k8, ks = quantize_qk(q, k, rotary)
+        else:
+            q8, qs = fp8_quantize_per_block(q, block_l=128)
+            k8, ks = fp8_quantize_per_block(k, block_l=128)
         v8, vs = fp8_quantize_per_head(v)
         if q.ndim == 3:
             q8, k8, v8 = q8[0], k8[0], v8[0]
         return PreparedFP8(q8, k8, v8, qs, ks, vs, layout, shape)
 
 
-def prepare_fp8_fused(q, k, v, *, cu_seqlens=None):
+def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
     """Three-kernel B200 preparation; returns V already in the packed layout.
 
     Dense single-sequence self-attention only, S >= 32768, D=128.  Optional contiguous int32 CUDA
-    metadata must contain [0, S]; the caller owns its values.
+    metadata must contain [0, S]; the caller owns its values.  ``rotary`` as for ``prepare_fp8``.
     """
     from .preparation import prepare_fp8_fused as implementation
 
-    return implementation(q, k, v, cu_seqlens=cu_seqlens)
+    return implementation(q, k, v, cu_seqlens=cu_seqlens, rotary=rotary)
 
 
 def attention_fp8(
@@ -179,6 +193,7 @@ def attention(
     mid_window_blocks=DEFAULT_MID_WINDOW_BLOCKS,
     return_lse=False,
     preparation="auto",
+    rotary=None,
 ):
     """BF16/FP16 in, BF16 attention out, FP8 quantisation included.
 
@@ -186,8 +201,11 @@ def attention(
     fuses preparation for eligible long single-sequence calls, ``'unfused'`` keeps the general
     preparation and ``'fused'`` requires the packed contract.  ``mode="bf16"`` belongs to the
     reference's second backend, which this build does not contain: it raises.
+    ``rotary`` (from ``rotary_plan``): Q and K are given as projected; the preparation normalises and rotates them.
     """
     validate_qkv(q, k, v)
+    if rotary is not None:
+        _check_rotary(rotary, q, k)
     if mode not in ("bf16", "expcast"):
         raise ValueError("mode must be bf16 or expcast")
     if (mode == "bf16") != (version == "reference"):
@@ -204,7 +222,7 @@ def attention(
             "S >= 32768, DSL 4.6.2, dense Open-VC ExpCast and no LSE"
         )
     return attention_fp8(
-        prepare_fp8_fused(q, k, v) if fuse else prepare_fp8(q, k, v),
+        prepare_fp8_fused(q, k, v, rotary=rotary) if fuse else prepare_fp8(q, k, v, rotary=rotary),
         version=version,
         causal=causal,
         softmax_scale=softmax_scale,

@@ -4,16 +4,19 @@ Host side of ovc_prepare_fused; mirrors prepare_fp8_fused of the reference
 (src/open_vc_attn/preparation.py:83-162): same validation and messages, same result layout.
 """
 
+import ctypes
+
 import torch
 
 from . import _lib
 
 
-def prepare_fp8_fused(q, k, v, *, cu_seqlens=None):
+def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
     """Prepare contiguous [S,H,128] or [1,S,H,128] self-attention for B200.
 
     Requires S >= 32768.  Pass existing int32 CUDA [0,S] metadata to have it reused by identity;
-    its values are the caller's contract.  Nothing here synchronises with the host.
+    its values are the caller's contract.  Nothing here synchronises with the host.  With ``rotary`` (from
+    ``rotary_plan``) Q and K are normalised and rotated in the launch that quantises them.
     """
     from .api import PreparedFP8, validate_qkv
 
@@ -24,6 +27,10 @@ def prepare_fp8_fused(q, k, v, *, cu_seqlens=None):
         raise ValueError("Fused preparation requires contiguous Q/K/V and S >= 32768")
     if torch.cuda.get_device_capability(q.device) != (10, 0):
         raise ValueError("Fused preparation is currently validated for B200 only")
+    if rotary is not None:
+        from .rotary import RotaryPlan
+
+        RotaryPlan.check(rotary, q, k)
     shape = tuple(q.shape)
     q, k, v = [t.reshape(-1, t.shape[-2], t.shape[-1]) for t in (q, k, v)]
     if cu_seqlens is not None and (
@@ -33,10 +40,10 @@ def prepare_fp8_fused(q, k, v, *, cu_seqlens=None):
         or not cu_seqlens.is_contiguous()
     ):
         raise ValueError("cu_seqlens must be contiguous int32 [0,S] on the QKV device")
-    return _prepare_packed(q, k, v, shape, cu_seqlens)
+    return _prepare_packed(q, k, v, shape, cu_seqlens, rotary)
 
 
-def _prepare_packed(q, k, v, shape, cu_seqlens=None):
+def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
     """The three launches, without the length/device policy checks (any S >= 1)."""
     from .api import PreparedFP8
 
@@ -54,14 +61,12 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None):
         packed = torch.empty((h, d, padded), dtype=torch.float8_e4m3fn, device=q.device)
         amax = torch.empty((1, h), dtype=torch.float32, device=q.device)
         vs = torch.empty((1, h), dtype=torch.float32, device=q.device)
-        _lib.check(
-            lib.ovc_prepare_fused(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), s, h, q8.data_ptr(),
-                k8.data_ptr(), packed.data_ptr(), qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), amax.data_ptr(),
-                _lib.stream_pointer(q.device),
-            ),
-            "ovc_prepare_fused",
-        )
+        outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)] + [_lib.stream_pointer(q.device)]
+        inputs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), s, h)
+        if rotary is None:
+            _lib.check(lib.ovc_prepare_fused(*inputs, *outputs), "ovc_prepare_fused")
+        else:
+            _lib.check(lib.ovc_prepare_fused_rotary(*inputs, ctypes.byref(rotary.arguments), *outputs), "ovc_prepare_fused_rotary")
         result = packed[..., :s].movedim(-1, 0)
         layout = dict(cu_seqlens_q=cu_seqlens, cu_seqlens_k=cu_seqlens, max_seqlen_q=s, max_seqlen_k=s)
         return PreparedFP8(q8, k8, result, qs, ks, vs, layout, shape, v_prepacked=True)

@@ -1,0 +1,243 @@
+"""Rotary positions with several axes, alone and inside the FP8 preparation, against the formula in 64 bits.
+
+Tolerances.  Every output is one rounding of a float32 value.  For that value each factor has a few float32 roundings: the
+norm (a sum of 128 squares, eight by eight and then four pairwise steps: at most 12 roundings of the sum, half of that after
+the root, rsqrtf 2 ulp, two products) under 12 * 2^-24 relative; cos and sin within 2^-24 * pi of the angle's rounding plus 2
+ulp of sincospif, under 6 * 2^-24 absolute; the two products and the sum 3 * 2^-24.  So |error| <= 24 * 2^-24 * hypot(a, b) * |w|
+max, for the pair (a, b) normalised, plus half a step of the output type (2^-8 bf16, 2^-11 fp16 relative to the value).
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from gpu_util import DEV  # noqa: E402
+
+F32 = 24 * 2.0 ** -24
+HALF_STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _ovc():
+    import open_vc_attn
+
+    return open_vc_attn
+
+
+def formula(x, positions, axes, interleaved=True, frequencies="axis", theta=10000.0, weight=None, eps=1e-6):
+    """([.., S, H, 128] float64 result, the length of each channel's pair, which bounds its float32 error)."""
+    x = x.double()
+    if weight is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * weight.double()
+    total, first, angles = sum(axes), 0, []
+    for a, d in enumerate(axes):
+        i = torch.arange(d // 2, device=x.device, dtype=torch.float64)
+        e = 2 * i / d if frequencies == "axis" else 2 * (first + i) / total
+        angles.append(positions[..., a].double()[..., None] * theta ** -e)
+        first += d // 2
+    t = torch.cat(angles, -1)[..., None, :]
+    i = torch.arange(total // 2, device=x.device)
+    at, to = (2 * i, 2 * i + 1) if interleaved else (i, i + 64)
+    y, size = x.clone(), x.abs()
+    a, b = x[..., at], x[..., to]
+    y[..., at], y[..., to] = a * t.cos() - b * t.sin(), a * t.sin() + b * t.cos()
+    size[..., at] = size[..., to] = torch.hypot(a, b)
+    return y, size
+
+
+def close(got, want, size):
+    off = (got.double() - want).abs()
+    limit = F32 * size + HALF_STEP[got.dtype] * want.abs() + (2.0 ** -24 if got.dtype == torch.float16 else 0.0)
+    limit = limit * (1 + 2.0 ** -7)  # the half step is relative to the value before it was rounded, off by the first term
+    assert bool((off <= limit).all()), float((off - limit).max())
+
+
+def inputs(shape_q, shape_k, seed, dtype):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    q, k = [torch.randn(s, generator=g, device=DEV).to(dtype) for s in (shape_q, shape_k)]
+    return q, k, [1 + 0.25 * torch.randn(128, generator=g, device=DEV) for _ in range(2)]
+
+
+CASES = [
+    # batch, tokens, q heads, k heads, axes, interleaved, frequencies, norm, type
+    (1, 1, 1, 1, (128,), False, "axis", True, torch.bfloat16),
+    (1, 1, 56, 56, (44, 42, 42), True, "axis", False, torch.float16),
+    (1, 17, 32, 8, (128,), False, "axis", True, torch.bfloat16),
+    (2, 129, 3, 1, (16, 56, 56), True, "axis", True, torch.float16),
+    (3, 77, 7, 7, (32, 48, 48), False, "head", True, torch.bfloat16),
+    (1, 1000, 28, 4, (40, 40, 40), True, "head", False, torch.bfloat16),
+    (1, 9001, 2, 2, (2, 2, 2, 2), True, "axis", True, torch.float16),
+    (2, 5000, 5, 9, (64, 64), False, "axis", False, torch.bfloat16),
+]
+
+
+@pytest.mark.parametrize("batch,s,hq,hk,axes,interleaved,frequencies,norm,dtype", CASES)
+@pytest.mark.parametrize("kind", ["int32", "int64", "float32", "per item"])
+def test_rotation_matches_the_formula(batch, s, hq, hk, axes, interleaved, frequencies, norm, dtype, kind):
+    ovc = _ovc()
+    q, k, (qw, kw) = inputs((batch, s, hq, 128), (batch, s, hk, 128), s + hq, dtype)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    lead = (batch, s) if kind == "per item" else (s,)
+    positions = torch.randint(0, 200000, (*lead, len(axes)), generator=g, device=DEV)
+    if kind == "float32":
+        positions = positions.float() / 7.0
+    elif kind != "int64":
+        positions = positions.int()
+    plan = ovc.rotary_plan(positions, axes=axes, interleaved=interleaved, frequencies=frequencies,
+                           q_weight=qw if norm else None, k_weight=kw if norm else None)
+    got = ovc.rotary_qk(q, k, plan)
+    for x, y, w in zip((q, k), got, (qw, kw)):
+        assert y.dtype == dtype and y.shape == x.shape and y.is_contiguous()
+        close(y, *formula(x, positions, axes, interleaved, frequencies, weight=w if norm else None))
+    again = ovc.rotary_qk(q, k, plan)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    if batch == 1 and kind != "per item":  # a 3-D call is the same sequence
+        assert all(torch.equal(a[0], b) for a, b in zip(got, ovc.rotary_qk(q[0], k[0], plan)))
+
+
+@pytest.mark.parametrize("s", [1, 40, 6000])
+def test_slices_of_a_fused_projection_and_other_strides(s):
+    ovc = _ovc()
+    g = torch.Generator(device=DEV).manual_seed(s)
+    qkv = torch.randn(2, s, 12, 128, generator=g, device=DEV).to(torch.bfloat16)
+    q, k = qkv[:, :, :6], qkv[:, :, 6:9]
+    positions = torch.arange(s, device=DEV)[:, None]
+    plan = ovc.rotary_plan(positions, axes=(128,))
+    dense = ovc.rotary_qk(q.contiguous(), k.contiguous(), plan)
+    assert all(torch.equal(a, b) for a, b in zip(ovc.rotary_qk(q, k, plan), dense))
+    heads_first = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k)]  # [B,H,S,128] storage
+    assert all(torch.equal(a, b) for a, b in zip(ovc.rotary_qk(*heads_first, plan), dense))
+    odd = torch.randn(2, s, 9, 129, generator=g, device=DEV).to(torch.bfloat16)[..., 1:]  # rows off the 16-byte grid: copied
+    assert all(torch.equal(a, b) for a, b in zip(ovc.rotary_qk(odd[:, :, :6], odd[:, :, 6:], plan),
+                                                 ovc.rotary_qk(odd[:, :, :6].contiguous(), odd[:, :, 6:].contiguous(), plan)))
+    one = q[:, :, :1].expand(2, s, 6, 128)  # one head shown six times
+    assert torch.equal(ovc.rotary_qk(one, k, plan)[0], ovc.rotary_qk(one.contiguous(), k, plan)[0])
+
+
+def test_special_values():
+    ovc = _ovc()
+    plan = ovc.rotary_plan(torch.zeros(4, 3, device=DEV, dtype=torch.int32), q_weight=torch.ones(128, device=DEV))
+    x = torch.zeros(4, 1, 128, device=DEV, dtype=torch.bfloat16)
+    x[1, 0, 5] = math.inf
+    x[2, 0, 6] = math.nan
+    x[3] = 3.0e38
+    q, k = ovc.rotary_qk(x, x, plan)
+    assert not q[0].any()  # 0 / sqrt(eps)
+    assert q[1:3].isnan().any(-1).all()
+    # a head that is not normalised and sits at position zero comes back bit for bit (a pair with an infinity has 0 * inf)
+    assert torch.equal(k[0], x[0]) and torch.equal(k[3], x[3])
+    text = ovc.grid_positions(2, 3, 4, text=5, start=(1, 0, 0), device=DEV)
+    assert text.shape == (29, 3) and not text[:5].any() and text[5].tolist() == [1, 0, 0] and text[-1].tolist() == [2, 2, 3]
+
+
+@pytest.mark.parametrize("batch,s,h,axes,interleaved,frequencies,norm,dtype", [
+    (1, 1, 1, (128,), False, "axis", True, torch.bfloat16),
+    (1, 127, 2, (44, 42, 42), True, "axis", True, torch.bfloat16),
+    (1, 129, 3, (32, 48, 48), False, "head", False, torch.float16),
+    (3, 300, 5, (16, 56, 56), True, "axis", True, torch.float16),
+    (1, 5000, 14, (40, 40, 40), True, "head", True, torch.bfloat16),
+    (1, 33001, 3, (44, 42, 42), True, "axis", True, torch.bfloat16),  # the fused preparation
+])
+def test_preparation_rotates_what_it_quantises(batch, s, h, axes, interleaved, frequencies, norm, dtype):
+    """Codes: E4M3 of value / descale: half a step (2^-4 relative, 2^-10 below the normal range) around the exact value, plus
+    the float32 error of the value (F32 of the pair's length) and of the scale.  Descales: the exact block maximum / 448,
+    within the float32 error of the largest value and of one division (div.full: 2 ulp)."""
+    ovc = _ovc()
+    shape = (batch, s, h, 128) if batch > 1 else (s, h, 128)
+    q, k, (qw, kw) = inputs(shape, shape, s, dtype)
+    v = torch.randn(shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)).to(dtype)
+    positions = torch.randint(0, 5000, (s, len(axes)), device=DEV, dtype=torch.int32, generator=torch.Generator(device=DEV).manual_seed(2))
+    plan = ovc.rotary_plan(positions, axes=axes, interleaved=interleaved, frequencies=frequencies,
+                           q_weight=qw if norm else None, k_weight=kw if norm else None)
+    fused = s >= 32768
+    got = (ovc.prepare_fp8_fused if fused else ovc.prepare_fp8)(q, k, v, rotary=plan)
+    plain = (ovc.prepare_fp8_fused if fused else ovc.prepare_fp8)(q, k, v)
+    blocks = -(-s // 128)
+    assert torch.equal(got.v.float(), plain.v.float()) and torch.equal(got.v_descale, plain.v_descale)
+    assert got.q_descale.shape == plain.q_descale.shape and got.k_descale.shape == plain.k_descale.shape
+    if got.q_descale.shape[-1] > blocks:
+        assert bool((got.q_descale[..., blocks:] == 1.0).all())
+    for x, w, codes, descale in ((q, qw, got.q, got.q_descale), (k, kw, got.k, got.k_descale)):
+        want, size = formula(x, positions, axes, interleaved, frequencies, weight=w if norm else None)
+        want, size = [t.view(batch, s, h, 128) for t in (want, size)]
+        pad = torch.nn.functional.pad(want.abs(), (0, 0, 0, 0, 0, blocks * 128 - s)).view(batch, blocks, 128, h, 128)
+        top = pad.amax((2, 4)).clamp_min(1e-12).transpose(1, 2)  # [B,H,blocks]
+        longest = torch.nn.functional.pad(size, (0, 0, 0, 0, 0, blocks * 128 - s)).view(batch, blocks, 128, h, 128).amax((2, 4)).transpose(1, 2)
+        d = descale.double()[..., :blocks]
+        assert bool(((d * 448 - top).abs() <= F32 * longest + 4 * 2.0 ** -24 * top).all())
+        per_token = d.transpose(1, 2).repeat_interleave(128, 1)[:, :s, :, None]
+        value, off = want / per_token, F32 * size / per_token + 4 * 2.0 ** -24 * (want / per_token).abs()
+        limit = (value.abs() * 2.0 ** -4).clamp_min(2.0 ** -10) + 1.1 * off
+        assert bool(((codes.double().view(batch, s, h, 128) - value).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("shape", [(777, 3), (2, 400, 4), (32769, 2)])
+def test_attention_rotates_as_a_call_of_its_own_does(shape):
+    """attention(rotary=plan) is attention_fp8 of the rotated preparation, bit for bit, and agrees with attention of
+    separately rotated Q and K: those were rounded to 16 bits in between, so a few codes differ by a step."""
+    ovc = _ovc()
+    shape = (*shape, 128)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q, k, v = [torch.randn(shape, generator=g, device=DEV).to(torch.bfloat16) for _ in range(3)]
+    s = shape[-3]
+    plan = ovc.rotary_plan(torch.stack([torch.arange(s, device=DEV)] * 3, -1), q_weight=torch.ones(128, device=DEV))
+    out = ovc.attention(q, k, v, rotary=plan)
+    fused = s >= 32768
+    prepared = (ovc.prepare_fp8_fused if fused else ovc.prepare_fp8)(q, k, v, rotary=plan)
+    assert torch.equal(out, ovc.attention_fp8(prepared))
+    apart = ovc.attention(*ovc.rotary_qk(q, k, plan), v)
+    assert float((out.float() - apart.float()).norm() / apart.float().norm()) < 2.0 ** -4 * 2  # two E4M3 half steps, Q and K
+
+
+def test_graph_capture_side_stream_and_concurrent_calls():
+    ovc = _ovc()
+    q, k, _ = inputs((500, 6, 128), (500, 2, 128), 4, torch.bfloat16)
+    positions = torch.arange(500, device=DEV)[:, None]
+    plan = ovc.rotary_plan(positions, axes=(128,))
+    want = ovc.rotary_qk(q, k, plan)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ovc.rotary_qk(q, k, plan)
+        same = ovc.rotary_qk(q, k, plan)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, other, same))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ovc.rotary_qk(q, k, plan)
+    fresh = torch.randn_like(q.float()).to(q.dtype)
+    q.copy_(fresh)
+    positions.add_(3)  # the plan refers to the caller's tensor
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(captured, ovc.rotary_qk(q, k, plan)))
+
+
+def test_refusals_on_the_device():
+    ovc = _ovc()
+    q, k, _ = inputs((8, 2, 128), (8, 2, 128), 1, torch.bfloat16)
+    plan = ovc.rotary_plan(torch.zeros(8, 3, device=DEV, dtype=torch.int32))
+    with pytest.raises(ValueError, match="7"):
+        ovc.rotary_qk(q[:7], k[:7], plan)
+    with pytest.raises(ValueError, match="same tokens"):
+        ovc.rotary_qk(q, k[:7], plan)
+    with pytest.raises(ValueError, match="matching dtypes"):
+        ovc.rotary_qk(q, k.half(), plan)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        ovc.rotary_qk(q.float(), k.float(), plan)
+    with pytest.raises(TypeError, match="rotary_plan"):
+        ovc.rotary_qk(q, k, object())
+    with pytest.raises(TypeError, match="rotary_plan"):
+        ovc.attention(q, k, k, rotary=torch.zeros(8, 3, device=DEV))
+    with pytest.raises(ValueError, match="same tokens"):
+        ovc.attention(q, k[:5], k[:5], rotary=plan)
+    with pytest.raises(ValueError, match="detach"):
+        ovc.rotary_qk(q.clone().requires_grad_(), k, plan)
+    with pytest.raises(ValueError, match="axes"):
+        ovc.rotary_plan(torch.zeros(8, 2, device=DEV, dtype=torch.int32))
+    with pytest.raises(ValueError, match="q_weight"):
+        ovc.rotary_plan(torch.zeros(8, 3, device=DEV, dtype=torch.int32), q_weight=torch.ones(64, device=DEV))
+    empty = ovc.rotary_qk(q[:0], k[:0], ovc.rotary_plan(torch.zeros(0, 3, device=DEV, dtype=torch.int32)))
+    assert empty[0].shape == (0, 2, 128)
