@@ -45,6 +45,8 @@ extern "C" {
 #define OVC_ATTN_CAUSAL 1     /* bottom-right aligned causal mask */
 #define OVC_ATTN_V_UNPACKED 2 /* v is [B,Sk,H,128] FP8 (the layout of the quantisers' output), not the packed one */
 
+#define OVC_ATTN_ZERO_TAIL 4  /* ovc_attention_packed: rows of out behind the last sequence are set to zero */
+
 #define OVC_STATUS_WAIT_EXPIRED 1u /* a bounded barrier wait gave up; the output rows of that launch hold NaN */
 
 int ovc_version(void);
@@ -274,6 +276,36 @@ int ovc_quantize_qk_rotary(const void* q, const void* k, int dtype, int64_t B, i
 int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H,
                              const ovc_rotary* rotary, void* q8, void* k8, void* v_packed, float* q_descale,
                              float* k_descale, float* v_descale, float* amax_ws, void* stream);
+
+/* ---- Attention over packed sequences in 16 bits ----
+ *
+ * Sequence b is rows cu_seqlens_q[b] .. cu_seqlens_q[b+1] of q and cu_seqlens_k[b] .. of k and v; Hq / Hk query heads
+ * share a key head (query head h reads key head h / (Hq / Hk)).  The 16-bit, packed, grouped-head counterpart of
+ * ovc_attention (the reference's kernel interface names the same options, cute/interface.py:110-179, its public
+ * functions use none of them).
+ *   q [Tq,Hq,128], k, v [Tk,Hk,128] f16/bf16 with strides[2] = elements from one token and one head to the next,
+ *       positive multiples of 8.
+ *   cu_seqlens_q, cu_seqlens_k [B+1] int32 on the DEVICE, 0 first, not decreasing.  Lengths may be zero.  Values outside
+ *       [0, T] or out of order give wrong rows but no access outside the tensors.
+ *   flags: OVC_ATTN_CAUSAL: token t of lq sees the keys below t + 1 + lk - lq; OVC_ATTN_ZERO_TAIL.
+ *   out [Tq,Hq,128] dense.  A row that sees no key is zero.  Rows behind the last sequence stay as they were unless
+ *       OVC_ATTN_ZERO_TAIL is given.
+ *   lse [Hq,Tq] f32 or NULL: natural logarithm of the sum of exponentials of the scaled scores, -inf for a row that
+ *       sees no key.
+ *   workspace: ovc_attention_packed_workspace() bytes, 16-byte aligned; NULL where that is 0.  Written before it is
+ *       read; one launch at a time may use it.
+ *   status: one uint32 on the device, OR-ed with OVC_STATUS_WAIT_EXPIRED by a launch whose bounded wait gave up; while it
+ *       is set, launches leave NaN and return.  host_status: pinned host memory that gets the same bit.  Both or
+ *       either may be NULL.
+ * 1 <= Hq / Hk <= 128; Tq, Tk <= 2^30; B <= 2^20.
+ */
+int ovc_attention_packed(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                         const int64_t* v_strides, int dtype, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int flags, float softmax_scale,
+                         void* out, float* lse, void* workspace, uint32_t* status, uint32_t* host_status, void* stream);
+
+/* Bytes of workspace for these sizes (0 for most: only launches with few query rows split the keys). */
+int64_t ovc_attention_packed_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk);
 
 /* ---- VC-Attention baseline: V-Smooth preparation and the mean-restoring attention variant ----
  *

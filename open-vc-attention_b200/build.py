@@ -13,7 +13,7 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
-SOURCES = ["prep.cu", "attn.cu", "vsmooth.cu", "rotary.cu"]
+SOURCES = ["prep.cu", "attn.cu", "vsmooth.cu", "rotary.cu", "packed.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",

@@ -32,12 +32,13 @@
 
 #include <atomic>
 
-#include <cuda.h>
 #include <cuda_bf16.h>
 #include <math.h>
 
 #include "common.cuh"
+#include "scores.cuh"
 #include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace ovc {
 namespace {
@@ -55,8 +56,6 @@ constexpr int kMeanSlice = 16;                    // key blocks restored by one 
 __host__ __device__ constexpr int ext_rows(bool vs) { return vs ? kMeanSlice : 8; }
 __host__ __device__ constexpr int pv_n(bool vs) { return kDim + ext_rows(vs); }  // 136 / 144
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 192, kColW = 480, kTmemCols = 512;
-constexpr long long kWaitCycles = 400000000LL;    // bounded barrier wait (~0.2 s)
-constexpr uint32_t kSleepHintNs = 100000;         // one hardware-suspended try_wait lasts at most this
 
 template <bool kVS, bool kVNat>
 struct SmemLayout {
@@ -115,28 +114,9 @@ __device__ __forceinline__ void give_up(volatile uint32_t* abort_flag, uint32_t*
     }
 }
 
-// Bounded wait.  The hardware suspends the thread inside try_wait while the phase is pending, so a
-// waiting warp issues almost nothing; the abort flag and the clock are looked at only every 16th
-// wake-up.  Returns false when the barrier did not complete in time or another thread of the CTA
-// already gave up; the caller then leaves its loop and the CTA tears down.
 __device__ __forceinline__ bool wait_bar(volatile uint32_t* abort_flag, uint64_t* bar, uint32_t parity, uint32_t* status,
                                          long long limit) {
-    const uint32_t addr = smem_addr(bar);
-    if (mbar_try_wait(addr, parity)) return true;
-    long long start = 0;
-#pragma unroll 1
-    for (uint32_t tries = 1;; ++tries) {
-        if (mbar_try_wait_sleep(addr, parity, kSleepHintNs)) return true;
-        if ((tries & 15u) == 0) {
-            if (*abort_flag) return false;
-            const long long now = clock64();
-            if (start == 0) start = now;
-            if (now - start > limit) {
-                give_up(abort_flag, status);
-                return false;
-            }
-        }
-    }
+    return wait_bounded(abort_flag, bar, parity, limit, [&] { give_up(abort_flag, status); });
 }
 
 template <class Layout>
@@ -169,18 +149,6 @@ __device__ __forceinline__ void qk_issue(uint32_t d_tmem, const uint64_t (&da)[4
         : "memory");
 }
 
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // bias = RD(-row_max * code_scale + 119.65 * 2^-24)
 __device__ __forceinline__ float expcast_bias(float row_max, float code_scale) {
     float b;
@@ -188,26 +156,10 @@ __device__ __forceinline__ float expcast_bias(float row_max, float code_scale) {
     return b;
 }
 
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // ExpCast codes of 128 scores: y = x*scale + bias in units of 2^-24 (one packed FMA per pair), rounded
 // to an FP16 subnormal whose low byte is the integer code (ReLU supplies the clamp at zero), low bytes
 // gathered four at a time.  Written stage by stage over 32 columns so that every stage is a run of
 // independent instructions.
-__device__ __forceinline__ uint64_t ffma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t pack_u2(uint32_t lo, uint32_t hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
 // Two FP16-subnormal conversions give (c2:c0) and (c3:c1) with each code in the low byte of a half;
 // one integer multiply-add (the FMA pipe, which has room) merges them into c0|c1<<8|c2<<16|c3<<24.
 __device__ __forceinline__ uint32_t codes4(uint64_t y01, uint64_t y23) {
@@ -228,27 +180,6 @@ __device__ __forceinline__ void encode128(const uint32_t (&s)[128], uint64_t sca
 #pragma unroll
         for (int i = 0; i < 8; ++i) codes[8 * c + i] = codes4(y[2 * i], y[2 * i + 1]);
     }
-}
-
-// Row max of 128 scores: a three-input max tree per 32 columns (the order in which a tensor-memory load fills
-// the registers), then the four partial results; 64 instructions.
-__device__ __forceinline__ float max32(const uint32_t* s) {
-    float a[11];
-#pragma unroll
-    for (int c = 0; c < 10; ++c)
-        a[c] = fmax3(__uint_as_float(s[3 * c]), __uint_as_float(s[3 * c + 1]), __uint_as_float(s[3 * c + 2]));
-    a[10] = fmaxf(__uint_as_float(s[30]), __uint_as_float(s[31]));
-    const float b0 = fmax3(a[0], a[1], a[2]), b1 = fmax3(a[3], a[4], a[5]), b2 = fmax3(a[6], a[7], a[8]);
-    return fmax3(fmax3(b0, b1, b2), a[9], a[10]);
-}
-__device__ __forceinline__ float max128(const uint32_t (&s)[128]) {
-    return fmaxf(fmax3(max32(s), max32(s + 32), max32(s + 64)), max32(s + 96));
-}
-
-__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
 }
 
 // After a failed wait: let the MMAs this thread has issued finish (bounded) before tensor memory is released.
@@ -922,22 +853,6 @@ __global__ void __launch_bounds__(256, 1) conversion_bench_kernel(uint32_t* sink
 }
 
 // ---- host side -------------------------------------------------------------------------------
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled_fn() {
-    static EncodeTiledFn fn = []() -> EncodeTiledFn {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult result;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) != cudaSuccess ||
-            result != cudaDriverEntryPointSuccess)
-            return nullptr;
-        return reinterpret_cast<EncodeTiledFn>(ptr);
-    }();
-    return fn;
-}
 
 // 4-D byte tensor (innermost first) with a 128-byte-swizzled box of box0 x box1 x 1 x 1.
 int make_map(CUtensorMap* map, const void* base, const cuuint64_t (&dims)[4], const cuuint64_t (&strides)[3],

@@ -1,0 +1,787 @@
+// Attention over packed sequences of different lengths in 16 bits: grouped query heads, optional causal mask, keys split
+// over CTAs where there are few query rows.  TMA -> shared memory -> tcgen05 (kind::f16) with accumulators in tensor
+// memory; the softmax on the CUDA cores in float32, in one pass over the keys with a running maximum and sum.
+//
+// A row of the score tile is one query head of one token: the G query heads of a key head are packed behind each other
+// (row = token * G + head in group), 128 / G tokens to a tile of 128 rows, so that a key tile is read once for all of them.
+//
+// A CTA runs two softmax stages of 128 rows each (one row per thread).  Whole: the stages hold neighbouring tiles of rows
+// and both visit every key tile.  Split: an item is a range of key tiles; the CTA writes unnormalised partial results that
+// combine_kernel joins.  Wide split has the stages of the whole form; narrow split (at most one tile of rows per sequence)
+// gives both stages the same rows and every other key tile, since with one tile of rows the time goes into reading keys.
+//
+// Warp roles (384 threads): warps 0-3 / 4-7 softmax of stage 0 / 1, warp 8 TMA loads, warp 9 the products, warps 10 and
+// 11 clear the CTA's share of the rows behind the last sequence, where asked to.  Warp 8 also
+// clears the rows of a value tile behind the end of its sequence (another sequence's values may be infinite or NaN, and
+// 0 times those is NaN).
+//
+// Tensor memory (512 columns): S0 0..127, S1 128..255, O0 256..383, O1 384..511.  The probabilities of a stage overwrite the
+// first 64 columns of its scores; the products of one thread run in the order of their issue, so S(n+1), issued behind
+// O += P(n) V(n), cannot overtake the reads of P(n), and a stage that sees S(n+1) knows O to be complete up to n.
+//
+// Shared memory: Q 2 x 32 KB, a ring of five 32 KB tiles that holds K and V alternately.
+
+#include <atomic>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "scores.cuh"
+#include "sm100_ptx.cuh"
+#include "tensor_map.cuh"
+
+namespace ovc {
+namespace {
+
+using namespace ptx;
+
+constexpr int kThreads = 384;
+constexpr int kSlots = 5;
+constexpr int kHalfBytes = kTile * 128;       // 128 rows of 64 values
+constexpr int kTileBytes = 2 * kHalfBytes;    // 128 rows of 128 values, as two halves of the channels
+constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
+constexpr int kMaxTiles = 512;                // row tiles that a split launch can plan (shared memory)
+
+enum Mode { kWhole = 0, kSplitWide = 1, kSplitNarrow = 2 };
+
+struct PackedParams {
+    const int* cu_q;       // [B+1]
+    const int* cu_k;       // [B+1]
+    void* out;             // [Tq,Hq,128]
+    float* lse;            // [Hq,Tq] or null
+    float* part_o;         // split: [items * Hk * 2][slot_rows][128], unnormalised
+    float2* part_ml;       // split: [items * Hk * 2][slot_rows], (maximum in units of log2, sum)
+    uint32_t* status;      // [1]: sticky word, or null
+    volatile uint32_t* host_status;
+    int B, Hq, Hk, G;
+    int tokens;            // tokens of a tile of 128 rows: 128 / G
+    int Tq, Tk;
+    int target, min_chunk; // split: wanted items per key head, least key tiles of an item
+    int max_tiles;         // split: row tiles that the workspace has room for
+    int slot_rows;
+    int zero_tail;         // rows behind the last sequence are set to zero
+    float scale_log2;
+};
+
+// What a CTA works on: rows of one sequence and a range of its key tiles.
+struct Item {
+    int valid;             // 0: no such item
+    int index;
+    int q0, lq, k0, lk;    // the sequence
+    int token0;            // first token of the tile within the sequence
+    int t0, t1;            // key tiles
+    int first, count;      // split: the items of this row tile
+    int q_end;             // end of the last sequence
+};
+
+__device__ __forceinline__ void bounds(const int* cu, int b, int total, int* start, int* length) {
+    const int lo = max(0, min(cu[b], total));
+    *start = lo;
+    *length = max(lo, min(cu[b + 1], total)) - lo;
+}
+
+// Key tiles that tokens [token0, token0 + n) of a sequence see.  Causal: the last token sees every key, token t the keys
+// below t + 1 + lk - lq.
+template <bool kCausal>
+__device__ __forceinline__ int visible_tiles(int lq, int lk, int token0, int n) {
+    int keys = lk;
+    if (kCausal) keys = max(0, min(lk, lk - lq + min(token0 + n, lq)));
+    return (keys + kTile - 1) / kTile;
+}
+
+__device__ __forceinline__ int warp_sum_before(int x, int lane, int* all) {
+    int s = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xFFFFFFFFu, s, o);
+        if (lane >= o) s += y;
+    }
+    *all = __shfl_sync(0xFFFFFFFFu, s, 31);
+    return s - x;
+}
+
+// Row tile `which` of the launch (one warp).  Within a sequence the last tokens come first: under a causal mask theirs are
+// the longest, and the short ones fill the SMs at the end.
+template <bool kCausal>
+__device__ void find_tile(const PackedParams& p, int per_tile, int which, int lane, Item* item) {
+    int before = 0;
+    bool found = false;
+    for (int base = 0; base < p.B && !found; base += 32) {
+        const int b = base + lane;
+        int q0 = 0, lq = 0;
+        if (b < p.B) bounds(p.cu_q, b, p.Tq, &q0, &lq);
+        const int n = (lq + per_tile - 1) / per_tile;
+        int all;
+        const int at = before + warp_sum_before(n, lane, &all);
+        if (which >= at && which < at + n) {
+            item->valid = 1, item->q0 = q0, item->lq = lq;
+            bounds(p.cu_k, b, p.Tk, &item->k0, &item->lk);
+            item->token0 = (n - 1 - (which - at)) * per_tile;
+            item->t0 = 0;
+            item->t1 = visible_tiles<kCausal>(lq, item->lk, item->token0, per_tile);
+        }
+        found = which < before + all;
+        before += all;
+    }
+    if (lane == 0) {
+        item->index = which;
+        if (!found) item->valid = 0;
+        item->q_end = max(0, min(p.cu_q[p.B], p.Tq));
+    }
+    __syncwarp();
+}
+
+// The plan of a split launch, made alike by every warp that asks: the key tiles of all row tiles are cut into pieces of
+// `chunk` (the same for all, so that long sequences get more CTAs than short ones and none waits for the longest), item
+// after item along the row tiles.  `which` counts items (by_item) or row tiles.
+struct PlanTile {
+    int seq, token0, key_tiles;
+};
+template <bool kCausal>
+__device__ void find_split(const PackedParams& p, int per_tile, int which, bool by_item, int lane, PlanTile* list, Item* item) {
+    int tiles = 0;
+    long long total = 0;
+    for (int base = 0; base < p.B; base += 32) {
+        const int b = base + lane;
+        int q0 = 0, lq = 0, k0 = 0, lk = 0;
+        if (b < p.B) {
+            bounds(p.cu_q, b, p.Tq, &q0, &lq);
+            bounds(p.cu_k, b, p.Tk, &k0, &lk);
+        }
+        // (More tiles than there is room for come of bounds that are out of order only.)
+        const int n = min((lq + per_tile - 1) / per_tile, kMaxTiles);
+        int all;
+        long long keys = 0;
+        const int at = tiles + warp_sum_before(n, lane, &all);
+        for (int i = 0; i < n && at + i < p.max_tiles; ++i) {
+            list[at + i] = PlanTile{b, i * per_tile, visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile)};
+            keys += list[at + i].key_tiles;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) keys += __shfl_xor_sync(0xFFFFFFFFu, keys, o);
+        total += keys;
+        tiles = min(tiles + all, p.max_tiles);
+    }
+    __syncwarp();
+    const int chunk = max(p.min_chunk, static_cast<int>((total + p.target - 1) / p.target));
+    int before = 0;
+    bool found = false;
+    for (int base = 0; base < tiles && !found; base += 32) {
+        const int t = base + lane;
+        const int n = t < tiles ? (list[t].key_tiles + chunk - 1) / chunk : 0;
+        int all;
+        const int at = before + warp_sum_before(n, lane, &all);
+        if (by_item ? which >= at && which < at + n : t == which && t < tiles) {
+            const PlanTile tile = list[t];
+            item->valid = 1;
+            bounds(p.cu_q, tile.seq, p.Tq, &item->q0, &item->lq);
+            bounds(p.cu_k, tile.seq, p.Tk, &item->k0, &item->lk);
+            item->token0 = tile.token0;
+            item->first = at, item->count = n;
+            item->t0 = (which - at) * chunk;
+            item->t1 = min(item->t0 + chunk, tile.key_tiles);
+        }
+        before += all;
+        found = by_item ? which < before : which < base + 32 && which < tiles;
+    }
+    if (lane == 0) {
+        item->index = which;
+        if (!found) item->valid = 0;
+        item->q_end = max(0, min(p.cu_q[p.B], p.Tq));
+    }
+    __syncwarp();
+}
+
+// Rows behind the last sequence: every CTA of a key head takes its share.
+__device__ __forceinline__ void clear_tail(const PackedParams& p, int q_end, int group0, int thread, int threads) {
+    for (long long t = q_end + static_cast<long long>(blockIdx.x); t < p.Tq; t += gridDim.x) {
+        uint4* dst = reinterpret_cast<uint4*>(p.out) + (t * p.Hq + group0) * 16;
+        for (int i = thread; i < p.G * 16; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
+        if (p.lse != nullptr)
+            for (int g = thread; g < p.G; g += threads) p.lse[static_cast<long long>(group0 + g) * p.Tq + t] = -INFINITY;
+    }
+}
+
+// ---- operands ----------------------------------------------------------------------------------------------------
+
+template <bool kBf16>
+__host__ __device__ constexpr uint32_t idesc(bool b_mn_major) {
+    return (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kSmemDescHi));
+    return d;
+}
+
+// S = Q K^T: both operands K-major, 64 channels to a half; eight steps of 16 channels (32 bytes).  One thread.
+__device__ __forceinline__ void product_qk(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t id) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t step = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "l"(desc(a_lo + step)), "l"(desc(b_lo + step)), "r"(id), "r"(k)
+            : "memory");
+    }
+}
+// O (+)= P V: P in tensor memory (two values per column), V as the MN-major operand (a row of shared memory is a key);
+// eight steps of 16 keys.  One thread.
+__device__ __forceinline__ void product_pv(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t id, bool accumulate) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_tmem + 8 * k), "l"(desc(b_lo + 128 * k)), "r"(id), "r"(k > 0 || accumulate ? 1 : 0)
+            : "memory");
+    }
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
+    uint32_t r;
+    if (kBf16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint64_t fadd2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float* a, float* b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+
+struct Smem {
+    alignas(1024) uint8_t q[2][kTileBytes];
+    alignas(1024) uint8_t ring[kSlots][kTileBytes];
+    alignas(8) uint64_t q_full[2];
+    uint64_t full[kSlots], empty[kSlots];  // a tile has landed / its last reader is done
+    uint64_t s_full[2];                    // the stage's scores are in tensor memory
+    uint64_t p_full[2];                    // the stage's probabilities are, and O is rescaled
+    uint64_t o_full[2];
+    uint64_t v_clean;                      // the rows behind the sequence's end are cleared in its last value tile
+    uint64_t drain;
+    uint32_t tmem_base;
+    volatile uint32_t abort_flag;
+};
+
+// The order in which a CTA visits key tiles.  Whole, wide: both stages every tile.  Narrow: stage s the tiles s, s + 2, ...
+// A tile is slot indices 2 i (K) and 2 i + 1 (V) of the ring, i counting the CTA's tiles.
+template <int kMode>
+__device__ __forceinline__ int tile_of(int stage, int n) {
+    return kMode == kSplitNarrow ? 2 * n + stage : n;
+}
+
+template <bool kBf16, bool kCausal, int kMode>
+__global__ void __launch_bounds__(kThreads, 1)
+packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+              const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PackedParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    __shared__ Item item;
+    __shared__ uint32_t gave_up;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kv_head = blockIdx.y;
+    const int per_cta = (kMode == kSplitNarrow ? 1 : 2) * p.tokens;  // tokens of a row tile
+
+    if (warp == 0) {
+        if (kMode == kWhole) find_tile<kCausal>(p, per_cta, blockIdx.x, lane, &item);
+        else find_split<kCausal>(p, per_cta, blockIdx.x, true, lane, reinterpret_cast<PlanTile*>(sm.q), &item);
+        // A barrier wait expired since the host last looked: start nothing, leave NaN.
+        if (lane == 0) gave_up = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
+    }
+    __syncthreads();
+    const int group0 = kv_head * p.G;  // first query head
+    const float nan = __int_as_float(0x7FC00000);
+
+    if (!item.valid) {  // an item beyond the last
+        if (kMode == kWhole && p.zero_tail) clear_tail(p, item.q_end, group0, threadIdx.x, kThreads);
+        return;
+    }
+
+    const int n_tiles = item.t1 - item.t0;
+    // Steps of each stage.
+    int steps[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        if (kMode == kSplitNarrow) {
+            steps[s] = (n_tiles - s + 1) / 2;
+        } else {
+            const int token = item.token0 + s * p.tokens;
+            steps[s] = token >= item.lq ? 0 : max(0, min(item.t1, visible_tiles<kCausal>(item.lq, item.lk, token, p.tokens)) - item.t0);
+        }
+    }
+    const bool run = n_tiles > 0 && gave_up == 0;
+    const auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return wait_bounded(&sm.abort_flag, bar, parity, kWaitCycles, [&] {
+            sm.abort_flag = 1;
+            if (p.status != nullptr) atomicOr(p.status, OVC_STATUS_WAIT_EXPIRED);
+            if (p.host_status != nullptr) {
+                *p.host_status = OVC_STATUS_WAIT_EXPIRED;
+                __threadfence_system();
+            }
+        });
+    };
+
+    uint32_t tmem = 0;
+    if (run) {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(smem_addr(&sm.q_full[i]), 1);
+                mbar_init(smem_addr(&sm.s_full[i]), 1);
+                mbar_init(smem_addr(&sm.p_full[i]), 128);
+                mbar_init(smem_addr(&sm.o_full[i]), 1);
+            }
+            for (int i = 0; i < kSlots; ++i) {
+                mbar_init(smem_addr(&sm.full[i]), 1);
+                mbar_init(smem_addr(&sm.empty[i]), 1);
+            }
+            mbar_init(smem_addr(&sm.v_clean), 1);
+            mbar_init(smem_addr(&sm.drain), 1);
+            sm.abort_flag = 0;
+            mbar_init_fence();
+        }
+        if (warp == 9) {
+            tmem_alloc(smem_addr(&sm.tmem_base), kTmemCols);
+            tmem_relinquish();
+        }
+        fence_proxy_async_smem();  // the plan was written where Q lands
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        tmem = sm.tmem_base;
+    }
+    // Keys of the last tile of this sequence; only an item that holds that tile has a value tile to clean.
+    const int last_tile = (item.lk + kTile - 1) / kTile - 1;
+    const int tail_rows = item.lk - last_tile * kTile;
+    const bool cleans = run && item.t1 - 1 == last_tile && tail_rows < kTile;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8 && run) {
+            // ---------------- TMA loads ----------------
+            const int q_tiles = kMode == kSplitNarrow ? 1 : 2;
+            int issued = 0;
+            if (lane == 0) {
+                tma_prefetch_desc(&tmap_k);
+                tma_prefetch_desc(&tmap_v);
+                const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
+                const uint64_t kv_policy = kMode == kSplitNarrow ? stream : keep;
+                const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128;  // of one half
+                for (int s = 0; s < q_tiles; ++s) {
+                    mbar_expect_tx(smem_addr(&sm.q_full[s]), 2 * q_bytes);
+                    const int token = item.q0 + item.token0 + s * p.tokens;
+                    for (int h = 0; h < 2; ++h)
+                        tma_load_4d(smem_addr(sm.q[s]) + h * kHalfBytes, &tmap_q, smem_addr(&sm.q_full[s]), 0, group0, token, h, stream);
+                }
+                for (int i = 0; i < 2 * n_tiles; ++i) {
+                    const int slot = i % kSlots;
+                    if (i >= kSlots && !wait(&sm.empty[slot], (i / kSlots - 1) & 1)) break;
+                    mbar_expect_tx(smem_addr(&sm.full[slot]), kTileBytes);
+                    const int key = item.k0 + (item.t0 + (i >> 1)) * kTile;
+                    tma_load_4d(smem_addr(sm.ring[slot]), (i & 1) ? &tmap_v : &tmap_k, smem_addr(&sm.full[slot]), 0, kv_head, key, 0, kv_policy);
+                    issued = i + 1;
+                }
+            }
+            issued = __shfl_sync(0xFFFFFFFFu, issued, 0);
+            // The last value tile: its rows behind the end of the sequence.  (The warp that issued the load may wait for
+            // it: its slot's earlier phases are over, so the parity is unambiguous.)
+            const int index = 2 * n_tiles - 1;
+            if (cleans && issued == 2 * n_tiles && __all_sync(0xFFFFFFFFu, wait(&sm.full[index % kSlots], (index / kSlots) & 1))) {
+                for (int h = 0; h < 2; ++h) {
+                    uint4* rows = reinterpret_cast<uint4*>(sm.ring[index % kSlots] + h * kHalfBytes);
+                    for (int i = tail_rows * 8 + lane; i < kTile * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_addr(&sm.v_clean));
+            }
+            // Every copy has landed before the CTA's shared memory goes away (it has, unless a wait expired).
+            if (lane == 0) {
+                const long long t0 = clock64();
+                for (int i = max(0, issued - kSlots); i < issued; ++i)
+                    while (!mbar_try_wait(smem_addr(&sm.full[i % kSlots]), (i / kSlots) & 1) && clock64() - t0 < kWaitCycles) {}
+                for (int s = 0; s < q_tiles; ++s)
+                    while (!mbar_try_wait(smem_addr(&sm.q_full[s]), 0) && clock64() - t0 < kWaitCycles) {}
+            }
+        } else if (warp == 9 && lane == 0 && run) {
+            // ---------------- products ----------------
+            constexpr uint32_t id_qk = idesc<kBf16>(false), id_pv = idesc<kBf16>(true);
+            const auto landed = [&](int index) { return wait(&sm.full[index % kSlots], (index / kSlots) & 1); };
+            const auto scores = [&](int s, int n) {
+                const int index = 2 * tile_of<kMode>(s, n);
+                if (!landed(index)) return false;
+                product_qk(tmem + kColS + 128 * s, smem_desc_lo(smem_addr(sm.q[kMode == kSplitNarrow ? 0 : s])),
+                           smem_desc_lo(smem_addr(sm.ring[index % kSlots])), id_qk);
+                commit(&sm.s_full[s]);
+                if (kMode == kSplitNarrow || s == 1 || n >= steps[1]) commit(&sm.empty[index % kSlots]);
+                return true;
+            };
+            bool ok = true;
+            for (int s = 0; ok && s < 2; ++s)
+                if (steps[s] > 0) ok = wait(&sm.q_full[kMode == kSplitNarrow ? 0 : s], 0) && scores(s, 0);
+            const int most = max(steps[0], steps[1]);
+            for (int n = 0; ok && n < most; ++n) {
+                for (int s = 0; ok && s < 2; ++s) {
+                    if (n >= steps[s]) continue;
+                    const int index = 2 * tile_of<kMode>(s, n) + 1;
+                    ok = landed(index) && (!cleans || tile_of<kMode>(s, n) != n_tiles - 1 || wait(&sm.v_clean, 0)) &&
+                         wait(&sm.p_full[s], n & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    product_pv(tmem + kColO + 128 * s, tmem + kColS + 128 * s,
+                               smem_desc_lo_bmn(smem_addr(sm.ring[index % kSlots]), kHalfBytes), id_pv, n > 0);
+                    if (n + 1 == steps[s]) commit(&sm.o_full[s]);
+                    if (kMode == kSplitNarrow || s == 1 || n >= steps[1]) commit(&sm.empty[index % kSlots]);
+                    if (n + 1 < steps[s]) ok = scores(s, n + 1);
+                }
+            }
+            if (!ok) {  // products in flight end before tensor memory is released
+                commit(&sm.drain);
+                const long long t0 = clock64();
+                while (!mbar_try_wait(smem_addr(&sm.drain), 0) && clock64() - t0 < kWaitCycles) {}
+            }
+        } else if (warp >= 10 && kMode == kWhole && p.zero_tail) {
+            clear_tail(p, item.q_end, group0, threadIdx.x - 320, 64);
+        }
+    } else {
+        // ---------------- softmax: one row per thread ----------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int stage = warp >> 2;
+        const int row = (warp & 3) * 32 + lane;
+        const int token = item.token0 + (kMode == kSplitNarrow ? 0 : stage * p.tokens) + row / p.G;  // within the sequence
+        const int head = group0 + row % p.G;
+        const bool real = row < p.tokens * p.G && token < item.lq;
+        const int keys = kCausal ? max(0, min(item.lk, item.lk - item.lq + token + 1)) : item.lk;
+        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+        const uint32_t t_s = lane_base + kColS + 128 * stage, t_o = lane_base + kColO + 128 * stage;
+        const int my_steps = run ? steps[stage] : 0;
+
+        float top = -INFINITY;     // the maximum that the accumulator is scaled by
+        float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
+        uint64_t sum2 = 0;         // the running sum, even and odd columns
+        bool ok = true;
+        for (int n = 0; n < my_steps; ++n) {
+            ok = __all_sync(0xFFFFFFFFu, wait(&sm.s_full[stage], n & 1));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[128];
+            tmem_ld32(t_s, s);
+            tmem_ld32(t_s + 32, s + 32);
+            tmem_ld32(t_s + 64, s + 64);
+            tmem_ld32(t_s + 96, s + 96);
+            tmem_wait_ld();
+            const int columns = keys - (item.t0 + tile_of<kMode>(stage, n)) * kTile;
+            if (__any_sync(0xFFFFFFFFu, columns < kTile)) {
+#pragma unroll
+                for (int c = 0; c < 128; ++c)
+                    if (c >= columns) s[c] = 0xFF800000u;  // -inf, whatever the key holds
+            }
+            // The maximum moves only when it grows by more than 2^8: until then probabilities above 1 are as exact as those
+            // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.
+            const float tile_top = max128(s);
+            float alpha = 1.0f;
+            if ((tile_top - top) * p.scale_log2 > 8.0f) {  // also the first finite maximum: top is -inf
+                alpha = ex2(fmaf(top, p.scale_log2, -tile_top * p.scale_log2));
+                top = tile_top;
+                shift = -top * p.scale_log2;
+                float a, b;
+                unpack2(sum2, &a, &b);
+                sum2 = pack2(a * alpha, b * alpha);
+            }
+            if (n > 0 && __any_sync(0xFFFFFFFFu, alpha < 1.0f)) {
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + 32 * c, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                    tmem_st32(t_o + 32 * c, o);
+                }
+            }
+            const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), shift2 = pack2(shift, shift);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t pr[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    uint64_t x = ffma2(pack_u2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, shift2);
+                    float a, b;
+                    unpack2(x, &a, &b);
+                    a = ex2(a), b = ex2(b);
+                    s[64 * c + 2 * e] = __float_as_uint(a), s[64 * c + 2 * e + 1] = __float_as_uint(b);
+                    pr[e] = narrow2<kBf16>(a, b);
+                }
+                tmem_st32(t_s + 32 * c, pr);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(smem_addr(&sm.p_full[stage]));
+            // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over.
+            uint64_t part[4] = {sum2, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 64; ++e) part[e & 3] = fadd2(part[e & 3], pack_u2(s[2 * e], s[2 * e + 1]));
+            sum2 = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
+        }
+        if (ok && my_steps > 0) ok = __all_sync(0xFFFFFFFFu, wait(&sm.o_full[stage], 0));
+        tc_fence_after();
+        ok = ok && gave_up == 0;
+        float a, b;
+        unpack2(sum2, &a, &b);
+        const float sum = ok ? a + b : nan;
+        if (kMode == kWhole) {
+            const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
+            if (real && p.lse != nullptr)
+                p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
+                    sum == 0.0f || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
+            uint4* dst = reinterpret_cast<uint4*>(p.out) + at * 16;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t o[32];
+                if (my_steps > 0 && ok) {  // warp-uniform
+                    tmem_ld32(t_o + 32 * c, o);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0;
+                }
+                if (real) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
+                        dst[4 * c + e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        } else {
+            const long long slot = ((static_cast<long long>(item.index) * p.Hk + kv_head) * 2 + stage) * p.slot_rows + row;
+            if (real) p.part_ml[slot] = make_float2(sum == 0.0f ? -INFINITY : -shift, sum);
+            float4* dst = reinterpret_cast<float4*>(p.part_o) + slot * 32;
+            if (my_steps > 0 && ok) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(t_o + 32 * c, o);
+                    tmem_wait_ld();
+                    if (real) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e)
+                            dst[8 * c + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                                         __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                    }
+                }
+            }
+        }
+    }
+    if (run) {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 9) {
+            tc_fence_after();
+            tmem_dealloc(tmem, kTmemCols);
+        }
+    }
+}
+
+// Joins the partial results of a split launch: a warp per row, four channels per lane.
+//   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i,  lse = ln 2 (M + log2 of that sum).
+// A partial that saw no key has l = 0 and its O was not written.
+template <bool kBf16, bool kCausal, bool kNarrow>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ PackedParams p) {
+    __shared__ Item item;
+    __shared__ PlanTile list[kMaxTiles];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kv_head = blockIdx.y, group0 = kv_head * p.G;
+    const int per_cta = (kNarrow ? 1 : 2) * p.tokens;
+    if (warp == 0) find_split<kCausal>(p, per_cta, blockIdx.x, false, lane, list, &item);
+    __syncthreads();
+    if (p.zero_tail && blockIdx.z == 0) clear_tail(p, item.q_end, group0, threadIdx.x, 256);
+    if (!item.valid) return;
+    const int rows = min(per_cta, item.lq - item.token0) * p.G;
+    for (int r = blockIdx.z * 8 + warp; r < rows; r += 8 * gridDim.z) {
+        // Row r of the row tile is row r of its only 128-row tile, or of the second one.
+        const int stage = kNarrow ? 0 : r / (p.tokens * p.G);
+        const int slot_row = r - stage * p.tokens * p.G;
+        const int parts = item.count * (kNarrow ? 2 : 1);
+        const auto slot = [&](int i) {
+            const int index = item.first + (kNarrow ? i >> 1 : i), s = kNarrow ? i & 1 : stage;
+            return ((static_cast<long long>(index) * p.Hk + kv_head) * 2 + s) * p.slot_rows + slot_row;
+        };
+        float top = -INFINITY;
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float sum = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < parts; ++i) {
+            const long long at = slot(i);
+            const float2 ml = p.part_ml[at];
+            if (ml.y == 0.0f) continue;
+            const float w = ml.y != ml.y ? ml.y : ex2(ml.x - top);
+            const float4 o = ml.y != ml.y ? make_float4(ml.y, ml.y, ml.y, ml.y) : __ldg(reinterpret_cast<const float4*>(p.part_o) + at * 32 + lane);
+            sum = fmaf(w, ml.y, sum);
+            acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
+        }
+        const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const long long t = item.q0 + item.token0 + r / p.G;
+        const int head = group0 + r % p.G;
+        reinterpret_cast<uint2*>(p.out)[(t * p.Hq + head) * 32 + lane] =
+            make_uint2(narrow2<kBf16>(acc.x * factor, acc.y * factor), narrow2<kBf16>(acc.z * factor, acc.w * factor));
+        if (p.lse != nullptr && lane == 0)
+            p.lse[static_cast<long long>(head) * p.Tq + t] = sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * 0.69314718055994531f;
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+// [tokens, heads, 128] of 16-bit values, read as (64 channels, heads, tokens, half) with a 128-byte-swizzled box.
+int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int64_t heads, int64_t token_stride, int64_t head_stride,
+             int box_heads, int box_tokens, int box_halves) {
+    const EncodeTiledFn fn = encode_tiled_fn();
+    if (fn == nullptr) return OVC_ERR_DRIVER;
+    const cuuint64_t dims[4] = {64, static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens), 2};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(head_stride) * 2, static_cast<cuuint64_t>(token_stride) * 2, 128};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens), static_cast<cuuint32_t>(box_halves)};
+    const cuuint32_t elem[4] = {1, 1, 1, 1};
+    const CUresult r = fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims,
+                          strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_last_cuda_error(static_cast<int>(r));
+        return OVC_ERR_DRIVER;
+    }
+    return OVC_OK;
+}
+
+// How a launch is laid out; from sizes alone (the lengths of the sequences are on the device).
+struct Layout {
+    int mode, tokens, slot_rows, target, min_chunk;
+    int64_t tiles;  // at most so many row tiles per key head
+    int64_t items;  // split: at most so many items per key head
+};
+
+Layout lay_out(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
+    constexpr int64_t kSms = 148;
+    Layout l{};
+    const int64_t G = Hq / Hk;
+    l.tokens = static_cast<int>(kTile / G);
+    // n sequences of at least one token make at most Tq tiles, and at most one tile each that is not full.
+    const auto tiles = [&](int64_t per_tile) { const int64_t t = Tq / per_tile + B; return t < Tq ? t : Tq; };
+    l.mode = kWhole, l.tiles = tiles(2 * l.tokens), l.items = l.tiles;
+    // Split where whole row tiles leave SMs without work and there are keys enough to share.
+    const int64_t key_tiles = ceil_div(Tk, kTile);
+    if (l.tiles * Hk < kSms && l.tiles <= kMaxTiles && key_tiles >= 4 * B) {
+        l.mode = kSplitWide;
+        if (Tq * G <= kTile * B && tiles(l.tokens) <= kMaxTiles) l.mode = kSplitNarrow, l.tiles = tiles(l.tokens);
+        l.target = static_cast<int>(ceil_div(2 * kSms, Hk));
+        l.min_chunk = 2;
+        l.items = l.target + l.tiles;
+        const int64_t rows = Tq * G;
+        l.slot_rows = static_cast<int>(rows < kTile ? rows : kTile);
+    }
+    return l;
+}
+
+int64_t workspace_bytes(const Layout& l, int64_t Hk) {
+    return l.mode == kWhole ? 0 : l.items * Hk * 2 * l.slot_rows * (kDim + 2) * static_cast<int64_t>(sizeof(float));
+}
+
+bool bad_sizes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
+    return B < 1 || Tq < 1 || Tk < 1 || Hk < 1 || Hk > 65535 || Hq < Hk || Hq % Hk != 0 || Hq / Hk > kTile || B > (1 << 20) ||
+           Tq > (1LL << 30) || Tk > (1LL << 30) || Hq > (1 << 20);
+}
+
+}  // namespace
+}  // namespace ovc
+
+using namespace ovc;
+
+extern "C" int64_t ovc_attention_packed_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
+    if (bad_sizes(B, Tq, Tk, Hq, Hk)) return 0;
+    return workspace_bytes(lay_out(B, Tq, Tk, Hq, Hk), Hk);
+}
+
+extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                                    const int64_t* v_strides, int dtype, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                    int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk, int flags, float softmax_scale, void* out,
+                                    float* lse, void* workspace, uint32_t* status, uint32_t* host_status, void* stream) {
+    if (bad_sizes(B, Tq, Tk, Hq, Hk) || !q || !k || !v || !q_strides || !k_strides || !v_strides || !cu_seqlens_q || !cu_seqlens_k || !out ||
+        (dtype != OVC_F16 && dtype != OVC_BF16) || (flags & ~(OVC_ATTN_CAUSAL | OVC_ATTN_ZERO_TAIL)) != 0 || !(softmax_scale > 0.0f) ||
+        !isfinite(softmax_scale) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
+        ((reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(cu_seqlens_k) | reinterpret_cast<uintptr_t>(lse)) & 3u))
+        return OVC_ERR_ARGUMENT;
+    for (const int64_t* s : {q_strides, k_strides, v_strides})
+        if (s[0] <= 0 || s[1] <= 0 || s[0] % 8 || s[1] % 8 || s[0] >= (1LL << 38) || s[1] >= (1LL << 38)) return OVC_ERR_ARGUMENT;
+    const Layout l = lay_out(B, Tq, Tk, Hq, Hk);
+    if (workspace_bytes(l, Hk) > 0 && (!workspace || !aligned16(workspace))) return OVC_ERR_ARGUMENT;
+
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    int major = 0, minor = 0;
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
+    if (err != cudaSuccess) { set_last_cuda_error(err); return OVC_ERR_CUDA; }
+    if (major != 10 || minor != 0) return OVC_ERR_UNSUPPORTED;
+
+    const bool bf16 = dtype == OVC_BF16, causal = (flags & OVC_ATTN_CAUSAL) != 0;
+    const int64_t G = Hq / Hk;
+    CUtensorMap map_q, map_k, map_v;
+    int rc = make_map(&map_q, q, bf16, Tq, Hq, q_strides[0], q_strides[1], static_cast<int>(G), l.tokens, 1);
+    if (rc == OVC_OK) rc = make_map(&map_k, k, bf16, Tk, Hk, k_strides[0], k_strides[1], 1, kTile, 2);
+    if (rc == OVC_OK) rc = make_map(&map_v, v, bf16, Tk, Hk, v_strides[0], v_strides[1], 1, kTile, 2);
+    if (rc != OVC_OK) return rc;
+
+    PackedParams p{};
+    p.cu_q = cu_seqlens_q, p.cu_k = cu_seqlens_k, p.out = out, p.lse = lse;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (l.mode == kWhole ? 0 : l.items * Hk * 2 * l.slot_rows * kDim));
+    p.status = status, p.host_status = host_status;
+    p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.Hk = static_cast<int>(Hk), p.G = static_cast<int>(G);
+    p.tokens = l.tokens, p.Tq = static_cast<int>(Tq), p.Tk = static_cast<int>(Tk);
+    p.target = l.target, p.min_chunk = l.min_chunk, p.max_tiles = static_cast<int>(l.tiles < kMaxTiles ? l.tiles : kMaxTiles), p.slot_rows = l.slot_rows;
+    p.zero_tail = (flags & OVC_ATTN_ZERO_TAIL) != 0;
+    p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
+
+    constexpr int smem = sizeof(Smem) + 1024;
+    auto s = static_cast<cudaStream_t>(stream);
+    const dim3 grid(static_cast<unsigned>(l.items), static_cast<unsigned>(Hk));
+    const auto launch = [&](auto kernel) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) { set_last_cuda_error(e); return static_cast<int>(OVC_ERR_CUDA); }
+        kernel<<<grid, kThreads, smem, s>>>(map_q, map_k, map_v, p);
+        return check_launch();
+    };
+    const auto by_mask = [&](auto is_bf16, auto is_causal) {
+        constexpr bool kB = decltype(is_bf16)::value, kC = decltype(is_causal)::value;
+        if (l.mode == kWhole) return launch(packed_kernel<kB, kC, kWhole>);
+        const int r = l.mode == kSplitNarrow ? launch(packed_kernel<kB, kC, kSplitNarrow>) : launch(packed_kernel<kB, kC, kSplitWide>);
+        if (r != OVC_OK) return r;
+        const int rows = (l.mode == kSplitNarrow ? 1 : 2) * l.tokens * static_cast<int>(G);
+        const int64_t rows_all = Tq * G < rows ? Tq * G : rows;
+        const dim3 cgrid(static_cast<unsigned>(l.tiles), static_cast<unsigned>(Hk), static_cast<unsigned>(ceil_div(rows_all, 8)));
+        if (l.mode == kSplitNarrow) combine_kernel<kB, kC, true><<<cgrid, 256, 0, s>>>(p);
+        else combine_kernel<kB, kC, false><<<cgrid, 256, 0, s>>>(p);
+        return check_launch();
+    };
+    if (bf16) return causal ? by_mask(std::true_type{}, std::true_type{}) : by_mask(std::true_type{}, std::false_type{});
+    return causal ? by_mask(std::false_type{}, std::true_type{}) : by_mask(std::false_type{}, std::false_type{});
+}

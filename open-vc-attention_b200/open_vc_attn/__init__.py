@@ -49,6 +49,12 @@ def raw_forward(*args, **kwargs):
     return implementation(*args, **kwargs)
 
 
+def attention_packed(*args, **kwargs):
+    from .packed import attention_packed as implementation
+
+    return implementation(*args, **kwargs)
+
+
 def rotary_plan(*args, **kwargs):
     from .rotary import rotary_plan as implementation
 
@@ -75,6 +81,7 @@ __all__ = [
     "prepare_v_repair",
     "attention_v_repair",
     "raw_forward",
+    "attention_packed",
     "rotary_plan",
     "grid_positions",
     "rotary_qk",

@@ -12,6 +12,7 @@ LIBRARY_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libovc.so")
 
 OVC_F16, OVC_BF16 = 0, 1
 OVC_ATTN_CAUSAL, OVC_ATTN_V_UNPACKED = 1, 2  # flags of ovc_attention_ex
+OVC_ATTN_ZERO_TAIL = 4  # and, with OVC_ATTN_CAUSAL, of ovc_attention_packed
 STATUS_WAIT_EXPIRED = 1
 
 _p, _i, _l, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float
@@ -44,6 +45,8 @@ SIGNATURES = {
     "ovc_selftest_wait": (_i, [_p, _l, _p, _p]),
     "ovc_copy_head_slice": (_i, [_p, _l, _l, _p, _l, _l, _l, _l, _l, _i, _p]),
     "ovc_attention_ex": (_i, [_p, _p, _p, _p, _l, _p, _p, _p, _l, _p, _p, _i, _l, _l, _l, _l, _f, _i, _p, _p]),
+    "ovc_attention_packed": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _l, _l, _l, _l, _l, _i, _f, _p, _p, _p, _p, _p, _p]),
+    "ovc_attention_packed_workspace": (_l, [_l, _l, _l, _l, _l]),
     "ovc_rotary_qk": (_i, [_p, _p, _p, _p, _i, _l, _l, _l, _l, _p, _p, _p, _p]),
     "ovc_quantize_qk_rotary": (_i, [_p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _l, _p, _l, _p]),
     "ovc_prepare_fused_rotary": (_i, [_p, _p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
