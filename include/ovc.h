@@ -248,8 +248,8 @@ typedef struct ovc_rotary {
     int64_t position_batch_stride;  /* in elements; 0: every batch item has the same positions */
     const double* turns;            /* HOST: 64 frequencies in turns per position (read during the call) */
     const uint8_t* pair_axis;       /* HOST: 64 axis indices < axes (read during the call) */
-    const float* q_weight;          /* device: [128] or null */
-    const float* k_weight;          /* device: [128] or null */
+    const float* q_weight;          /* device: [128], 16-byte aligned, or null */
+    const float* k_weight;          /* device: [128], 16-byte aligned, or null */
     int position_type;              /* OVC_POSITIONS_* */
     int axes;                       /* 1 .. 64 */
     int half_split;
@@ -265,12 +265,14 @@ int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const 
                   int64_t S, int64_t Hq, int64_t Hk, const ovc_rotary* rotary, void* q_out, void* k_out, void* stream);
 
 /*
- * ovc_quantize_per_block of rotated (and normalised) Q and K, both in one launch.  The rotated values are not rounded
- * to 16 bits in between.  q, k dense [B,S,H,128].
+ * ovc_quantize_per_block of rotated (and normalised) Q and K and ovc_quantize_per_head of V, in three launches.  The
+ * rotated values are not rounded to 16 bits in between.
+ *   q, k, v dense [B,S,H,128]; q8, k8, v8 the same in fp8; q_descale, k_descale [B,H,ceil(S/128)], v_descale [B,H];
+ *   amax_ws [B,H] f32 scratch (holds the per-head max |v| afterwards).
  */
-int ovc_quantize_qk_rotary(const void* q, const void* k, int dtype, int64_t B, int64_t S, int64_t H,
-                           const ovc_rotary* rotary, void* q8, void* k8, float* q_descale, int64_t q_descale_stride,
-                           float* k_descale, int64_t k_descale_stride, void* stream);
+int ovc_prepare_rotary(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t S, int64_t H,
+                       const ovc_rotary* rotary, void* q8, void* k8, void* v8, float* q_descale, float* k_descale,
+                       float* v_descale, float* amax_ws, void* stream);
 
 /* ovc_prepare_fused with rotated (and normalised) Q and K. */
 int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H,

@@ -25,6 +25,10 @@ inline int check_launch() {
 int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, float* amax_ws, void* v_packed, float* v_descale,
                             void* stream);
 
+// The same with row-major codes, for a batch.
+int launch_amax_cast_v(const void* v, int dtype, int64_t B, int64_t S, int64_t H, float* amax_ws, void* codes, float* v_descale,
+                       void* stream);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 constexpr int kTile = 128;  // tokens per quantisation block and per key tile

@@ -400,6 +400,22 @@ int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, floa
     return check_launch();
 }
 
+int launch_amax_cast_v(const void* v, int dtype, int64_t B, int64_t S, int64_t H, float* amax_ws, void* codes, float* v_descale,
+                       void* stream) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(S, kTile)), static_cast<unsigned>(H), static_cast<unsigned>(B));
+    const int h = static_cast<int>(H);
+    auto s = static_cast<cudaStream_t>(stream);
+    auto* c = static_cast<uint8_t*>(codes);
+    if (dtype == OVC_BF16) {
+        head_amax_kernel<OVC_BF16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
+        head_cast_kernel<OVC_BF16, false><<<grid, 128, 0, s>>>(v, amax_ws, c, v_descale, nullptr, S, h);
+    } else {
+        head_amax_kernel<OVC_F16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
+        head_cast_kernel<OVC_F16, false><<<grid, 128, 0, s>>>(v, amax_ws, c, v_descale, nullptr, S, h);
+    }
+    return check_launch();
+}
+
 }  // namespace ovc
 
 extern "C" {

@@ -5,15 +5,23 @@
 //   y = turn(x * w / sqrt(mean(x^2) + eps)),   (a, b) -> (a cos t - b sin t, a sin t + b cos t) for each pair of channels,
 //   t = position[axis of the pair] * frequency of the pair.
 //
-// Angles.  A float32 product position * frequency is off by 2^-24 of itself: 2e-3 radians at position 30000.  So the
-// product is taken in float64 in units of whole turns, its fractional part (exact) rounded to float32, and sincospif gives
-// both functions: off by about 2e-7 whatever the position.  A head is 64 pairs, so a token costs 64 double products and
-// 64 sincospif, shared by all its heads; everything else is float32, rounded once when it is stored.
+// Angles.  A float32 product position * frequency is off by 2^-24 of itself: 2e-3 radians at position 30000.  Only the
+// fraction of a turn counts, so a frequency is an integer in units of 2^-64 turns and the product with a position is
+// taken modulo 2^64, which drops the whole turns exactly; its upper 32 bits go to sincospif.  The angle is off by about
+// 2e-7 whatever the position, without an instruction in float64.  A token has 64 pairs, shared by all its heads;
+// everything else is float32, rounded once when it is stored.
+//
+// A lane holds four pairs of one head and sixteen lanes a head, in both layouts of the pairs (neighbours: 16 bytes in a
+// row; halves: 8 bytes from each half of the head), so no value of a pair crosses lanes and both pair members are
+// computed two at a time (f32x2).
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "rows.cuh"
+#include "scores.cuh"
 
 namespace ovc {
 namespace {
@@ -25,53 +33,165 @@ struct Angles {
     long long batch_stride; // in elements; 0: the same positions for every batch item
     int type, axes;
     float eps;
-    double turns[kPairs];   // frequency / 2 pi of each pair; 0 leaves the pair as it is
+    unsigned long long turns[kPairs];  // per position, in units of 2^-64 turns; 0 leaves the pair as it is
     uint8_t axis[kPairs];
 };
 
-// cos and sin of one pair at one token.
-__device__ __forceinline__ float2 pair_turn(const Angles& a, long long row, int pair) {
-    const double f = a.turns[pair];
-    const long long at = row + a.axis[pair];
-    double pos;
-    if (a.type == OVC_POSITIONS_I32) pos = static_cast<double>(__ldg(static_cast<const int*>(a.positions) + at));
-    else if (a.type == OVC_POSITIONS_I64) pos = static_cast<double>(__ldg(static_cast<const long long*>(a.positions) + at));
-    else pos = static_cast<double>(__ldg(static_cast<const float*>(a.positions) + at));
-    const double turns = f == 0.0 ? 0.0 : pos * f;
-    float s, c;
-    sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-    return make_float2(c, s);
+// position * turns modulo one turn, in units of 2^-64, for a float32 position m * 2^e.
+__device__ __forceinline__ unsigned long long float_turns(float position, unsigned long long turns) {
+    const uint32_t bits = __float_as_uint(position);
+    const int field = (bits >> 23) & 255;
+    if (field == 0) return 0;  // zero (a subnormal position turns nothing)
+    const unsigned long long m = (bits & 0x7FFFFFu) | 0x800000u;
+    const unsigned long long lo = m * turns, hi = __umul64hi(m, turns);
+    const int e = field - 150;
+    unsigned long long x;
+    if (e >= 0) x = e < 64 ? lo << e : 0;
+    else if (e > -64) x = (lo >> -e) | (hi << (64 + e));
+    else x = e > -128 ? hi >> (-e - 64) : 0;
+    return bits >> 31 ? 0 - x : x;
 }
 
-// Eight channels 8 * c16 .. of one head, sixteen lanes to a head.  kHalf: channel i is paired with channel i + 64, held
-// by lane c16 ^ 8, and cs[e] belongs to channel 8 * (c16 & 7) + e; otherwise neighbours are paired and cs[0..3] are used.
-// `lanes`: the sixteen lanes of the head.
-template <bool kHalf>
-__device__ __forceinline__ void norm_turn(float (&x)[8], const float* w, float eps, const float2* cs, int c16, uint32_t lanes) {
-    if (w != nullptr) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(lanes, sum, o);
-        const float r = rsqrtf(fmaf(sum, 1.0f / kDim, eps));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-    }
-    if (kHalf) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float other = __shfl_xor_sync(lanes, x[i], 8);
-            x[i] = fmaf(x[i], cs[i].x, (c16 < 8 ? -other : other) * cs[i].y);
-        }
+// The frequencies in shared memory: lanes want different pairs, and the parameters' constant bank serves one address at
+// a time (read from there, the angles took twice as long as everything else).
+struct Pairs {
+    unsigned long long turns[kPairs];
+    uint8_t axis[kPairs];
+};
+__device__ __forceinline__ void stage_pairs(const Angles& a, Pairs& pairs) {
+    if (threadIdx.x < kPairs) pairs.turns[threadIdx.x] = a.turns[threadIdx.x], pairs.axis[threadIdx.x] = a.axis[threadIdx.x];
+}
+
+// cos and sin of one pair at one token, whose positions start at `row`.
+__device__ __forceinline__ float2 pair_turn(const Angles& a, const Pairs& pairs, long long row, int pair) {
+    const unsigned long long f = pairs.turns[pair];
+    const long long at = row + pairs.axis[pair];
+    unsigned long long x;
+    bool finite = true;
+    if (a.type == OVC_POSITIONS_I32) {
+        x = static_cast<unsigned long long>(static_cast<long long>(__ldg(static_cast<const int*>(a.positions) + at))) * f;
+    } else if (a.type == OVC_POSITIONS_I64) {
+        x = static_cast<unsigned long long>(__ldg(static_cast<const long long*>(a.positions) + at)) * f;
     } else {
+        const float position = __ldg(static_cast<const float*>(a.positions) + at);
+        finite = isfinite(position) || f == 0;
+        x = f == 0 ? 0 : float_turns(position, f);
+    }
+    float s, c;
+    sincospif(static_cast<float>(static_cast<int>((x + 0x80000000ull) >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31 half turns
+    return finite ? make_float2(c, s) : make_float2(NAN, NAN);
+}
+
+__device__ __forceinline__ uint64_t fmul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ void split2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+
+// Four pairs (a, b): first members a01, a23, second members b01, b23.
+struct Four {
+    uint64_t a[2], b[2];
+};
+
+// 16-bit words: with kHalf x and y are the first members, z and w the second; otherwise a word is a pair.
+template <int DT, bool kHalf>
+__device__ __forceinline__ Four widen_pairs(const uint4& raw) {
+    float f[8];
+    widen8<DT>(raw, f);
+    Four v;
+    if (kHalf) v.a[0] = pack2(f[0], f[1]), v.a[1] = pack2(f[2], f[3]), v.b[0] = pack2(f[4], f[5]), v.b[1] = pack2(f[6], f[7]);
+    else v.a[0] = pack2(f[0], f[2]), v.a[1] = pack2(f[4], f[6]), v.b[0] = pack2(f[1], f[3]), v.b[1] = pack2(f[5], f[7]);
+    return v;
+}
+// The values in the order of the stored channels.
+template <bool kHalf>
+__device__ __forceinline__ void in_order(const Four& v, float (&f)[8]) {
+    float a[4], b[4];
+    split2(v.a[0], a[0], a[1]), split2(v.a[1], a[2], a[3]), split2(v.b[0], b[0], b[1]), split2(v.b[1], b[2], b[3]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = x[2 * i], b = x[2 * i + 1];
-            x[2 * i] = fmaf(a, cs[i].x, -b * cs[i].y);
-            x[2 * i + 1] = fmaf(a, cs[i].y, b * cs[i].x);
+    for (int i = 0; i < 4; ++i) {
+        f[kHalf ? i : 2 * i] = a[i];
+        f[kHalf ? 4 + i : 2 * i + 1] = b[i];
+    }
+}
+// (The library wants weights on a 16-byte boundary.)
+template <bool kHalf>
+__device__ __forceinline__ Four load_weights(const float* weight, int c16) {
+    const float4 x = reinterpret_cast<const float4*>(weight)[kHalf ? c16 : 2 * c16];
+    const float4 y = reinterpret_cast<const float4*>(weight)[kHalf ? c16 + 16 : 2 * c16 + 1];
+    Four v;
+    if (kHalf) v.a[0] = pack2(x.x, x.y), v.a[1] = pack2(x.z, x.w), v.b[0] = pack2(y.x, y.y), v.b[1] = pack2(y.z, y.w);
+    else v.a[0] = pack2(x.x, x.z), v.a[1] = pack2(y.x, y.z), v.b[0] = pack2(x.y, x.w), v.b[1] = pack2(y.y, y.w);
+    return v;
+}
+// This lane's eight channels of a head.
+template <bool kHalf>
+__device__ __forceinline__ uint4 load_head(const uint16_t* head, int c16) {
+    if (!kHalf) return ld_stream(head + 8 * c16);
+    uint4 r;
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(head + 4 * c16));
+    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.z), "=r"(r.w) : "l"(head + 4 * c16 + 64));
+    return r;
+}
+
+__device__ __forceinline__ float squares(const Four& v) {
+    uint64_t sum = fmul2(v.a[0], v.a[0]);
+    sum = ffma2(v.a[1], v.a[1], sum);
+    sum = ffma2(v.b[0], v.b[0], sum);
+    sum = ffma2(v.b[1], v.b[1], sum);
+    float x, y;
+    split2(sum, x, y);
+    return x + y;
+}
+__device__ __forceinline__ void times(Four& v, const Four& w) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v.a[i] = fmul2(v.a[i], w.a[i]), v.b[i] = fmul2(v.b[i], w.b[i]);
+}
+struct Turns {
+    uint64_t c[2], s[2], minus_s[2];
+};
+__device__ __forceinline__ Turns make_turns(const float4& c, const float4& s) {
+    return Turns{{pack2(c.x, c.y), pack2(c.z, c.w)}, {pack2(s.x, s.y), pack2(s.z, s.w)}, {pack2(-s.x, -s.y), pack2(-s.z, -s.w)}};
+}
+__device__ __forceinline__ void turn(Four& v, const Turns& t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t a = v.a[i], b = v.b[i];
+        v.a[i] = ffma2(a, t.c[i], fmul2(b, t.minus_s[i]));
+        v.b[i] = ffma2(a, t.s[i], fmul2(b, t.c[i]));
+    }
+}
+
+// Sums over the sixteen lanes of a head for N = 2, 4 or 8 heads at once: steps in which a lane gives half of its sums away and
+// adds up the other half, so that 4 sums cost 5 exchanges instead of 16.  Lane lane_of_sum<N>(i) is left with sum i.
+template <int N>
+__device__ __forceinline__ constexpr int lane_of_sum(int i) { return i * (16 / N); }
+template <int N>
+__device__ __forceinline__ float sums_of_heads(float (&v)[N], int c16) {
+    int o = 8;
+#pragma unroll
+    for (int n = N / 2; n >= 1; n >>= 1, o >>= 1) {
+        const bool up = c16 & o;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, o);
         }
     }
+    float sum = v[0];
+#pragma unroll
+    for (int last = 8 / N; last > 0; last >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, last);
+    return sum;
+}
+// 1 / sqrt(mean(x^2) + eps) of N heads.
+template <int N>
+__device__ __forceinline__ void norm_factors(const Four (&v)[N], float eps, int c16, float (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = squares(v[i]);
+    const float mine = rsqrtf(fmaf(sums_of_heads<N>(r, c16), 1.0f / kDim, eps));
+#pragma unroll
+    for (int i = 0; i < N; ++i) r[i] = __shfl_sync(0xFFFFFFFFu, mine, lane_of_sum<N>(i), 16);
 }
 
 template <int DT>
@@ -100,115 +220,202 @@ struct RotaryArgs {
     float* amax_init;                    // rotary_quant_kernel: optional [H], set to 0
 };
 
-constexpr int kRowsAhead = 4;  // heads that a half warp has in flight
+constexpr int kUnitRows = 32, kUnitWarps = 4, kGroupRows = 8;
 
-// HBM bound: 4 bytes per element (2 read, 2 written).  Sixteen lanes hold a head (16 bytes each), a CTA is sixteen such
-// half warps: `token_tile` of them on tokens of their own, the others on further heads of the same tokens, so that a lane
-// computes its four (or eight) angles once and keeps them in registers for all heads it visits.  gridDim.y splits the heads
-// where there are few tokens.
-template <int DT, bool kHalf>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryArgs a, int token_tile, int rows_per_cta) {
-    const int c16 = threadIdx.x & 15, half_warp = threadIdx.x >> 4;
-    const uint32_t lanes = 0xFFFFu << (threadIdx.x & 16);
-    const long long token = static_cast<long long>(blockIdx.x) * token_tile + half_warp % token_tile;
-    if (token >= a.tokens) return;
-    const int step = 16 / token_tile;
+// 16 bytes to shared memory behind the thread's back: what is in flight takes no registers.
+__device__ __forceinline__ void copy16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+template <int kPending>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// HBM bound: 4 bytes per element (2 read, 2 written).  A warp takes up to 32 heads of one token (those of q, then those of
+// k), asks for all of them at once, computes the token's angles meanwhile - four pairs to a lane, kept in registers - and
+// then works through the heads eight at a time, two side by side, as they arrive.
+template <int DT, bool kHalf, bool kNorm>
+__global__ void __launch_bounds__(32 * kUnitWarps, 7) rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_rows, int units) {
+    extern __shared__ __align__(16) uint8_t staged[];
+    __shared__ Pairs pairs;
+    __shared__ __align__(16) float weights[2][kDim];
+    const int lane = threadIdx.x & 31, c16 = lane & 15, side = lane >> 4;
+    const long long unit = static_cast<long long>(blockIdx.x) * kUnitWarps + (threadIdx.x >> 5);
+    const long long wanted = unit / units, token = min(wanted, a.tokens - 1);
     const long long b = token / a.S, s = token - b * a.S;
+    const int q_heads = a.src[0].heads;
+    const int first = static_cast<int>(unit - wanted * units) * unit_rows;
+    const int rows = wanted < a.tokens ? min(unit_rows, q_heads + a.src[1].heads - first) : 0;
+    uint8_t* const mine = staged + (threadIdx.x >> 5) * unit_rows * 256;
 
-    float2 cs[kHalf ? 8 : 4];
+    const uint16_t* const xq = a.src[0].x + b * a.src[0].batch + s * a.src[0].token + 8 * c16;
+    const uint16_t* const xk = a.src[1].x + b * a.src[1].batch + s * a.src[1].token + 8 * c16;
 #pragma unroll
-    for (int i = 0; i < (kHalf ? 8 : 4); ++i)
-        cs[i] = pair_turn(a.angles, b * a.angles.batch_stride + s * a.angles.axes, kHalf ? 8 * (c16 & 7) + i : 4 * c16 + i);
-
-    // The heads of q and then those of k are one list; this CTA has [first, last) of it.
-    const int first = blockIdx.y * rows_per_cta;
-    const int last = min(first + rows_per_cta, a.src[0].heads + a.src[1].heads);
-#pragma unroll 1
-    for (int which = 0; which < 2; ++which) {
-        const Source& t = a.src[which];
-        const int before = which == 0 ? 0 : a.src[0].heads;
-        const int end = min(last - before, t.heads);
-        const uint16_t* x = t.x + b * t.batch + s * t.token + c16 * 8;
-        uint4* y = reinterpret_cast<uint4*>(t.y) + token * t.heads * (kDim / 8) + c16;
-        float w[8];
-        if (t.weight != nullptr) {
+    for (int g = 0; g < kUnitRows; g += kGroupRows) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __ldg(t.weight + c16 * 8 + i);
+        for (int i = 0; i < kGroupRows; i += 2) {
+            const int row = g + i + side, h = first + row;
+            if (row < rows) copy16(mine + row * 256 + 16 * c16, h < q_heads ? xq + h * a.src[0].head : xk + (h - q_heads) * a.src[1].head);
         }
-        for (int h = max(first - before, 0) + half_warp / token_tile; h < end; h += kRowsAhead * step) {
-            uint4 raw[kRowsAhead];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    stage_pairs(a.angles, pairs);
+    if (kNorm) {
+        for (int i = threadIdx.x; i < 2 * kDim; i += 32 * kUnitWarps) {
+            const float* weight = a.src[i / kDim].weight;
+            weights[i / kDim][i % kDim] = weight != nullptr ? __ldg(weight + i % kDim) : 1.0f;
+        }
+    }
+    __syncthreads();
+    if (rows == 0) return;
+    // Either half of the warp computes two of a lane's four angles.
+    float cs[4], sn[4];
 #pragma unroll
-            for (int u = 0; u < kRowsAhead; ++u)
-                if (h + u * step < end) raw[u] = ld_stream(x + (h + u * step) * t.head);
+    for (int i = 0; i < 2; ++i) {
+        const float2 t = pair_turn(a.angles, pairs, b * a.angles.batch_stride + s * a.angles.axes, 4 * c16 + 2 * side + i);
+        const float c = __shfl_xor_sync(0xFFFFFFFFu, t.x, 16), s = __shfl_xor_sync(0xFFFFFFFFu, t.y, 16);
+        cs[i] = side ? c : t.x, cs[2 + i] = side ? t.x : c;
+        sn[i] = side ? s : t.y, sn[2 + i] = side ? t.y : s;
+    }
+    const Turns turns = make_turns(make_float4(cs[0], cs[1], cs[2], cs[3]), make_float4(sn[0], sn[1], sn[2], sn[3]));
+    uint16_t* const yq = static_cast<uint16_t*>(a.src[0].y) + token * q_heads * kDim;
+    uint16_t* const yk = static_cast<uint16_t*>(a.src[1].y) + token * a.src[1].heads * kDim;
+
+    const auto group = [&](int g) {
+        constexpr int kRows = kGroupRows / 2;
+        Four v[kRows];
 #pragma unroll
-            for (int u = 0; u < kRowsAhead; ++u) {
-                if (h + u * step >= end) break;
-                float f[8];
-                widen8<DT>(raw[u], f);
-                norm_turn<kHalf>(f, t.weight != nullptr ? w : nullptr, a.angles.eps, cs, c16, lanes);
-                y[static_cast<long long>(h + u * step) * (kDim / 8)] =
-                    make_uint4(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]), narrow2<DT>(f[4], f[5]), narrow2<DT>(f[6], f[7]));
+        for (int i = 0; i < kRows; ++i) {
+            const uint8_t* from = mine + min(g + 2 * i + side, rows - 1) * 256;
+            uint4 raw;
+            if (kHalf) {
+                const uint2 lo = *reinterpret_cast<const uint2*>(from + 8 * c16), hi = *reinterpret_cast<const uint2*>(from + 8 * c16 + 128);
+                raw = make_uint4(lo.x, lo.y, hi.x, hi.y);
+            } else {
+                raw = *reinterpret_cast<const uint4*>(from + 16 * c16);
+            }
+            v[i] = widen_pairs<DT, kHalf>(raw);
+        }
+        float r[kRows];
+        if (kNorm) norm_factors<kRows>(v, a.angles.eps, c16, r);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int row = g + 2 * i + side, h = first + row;
+            if (kNorm) {
+                // (A tensor without weights is multiplied by 1 and 1.)
+                const float k = a.src[h < q_heads ? 0 : 1].weight != nullptr ? r[i] : 1.0f;
+                const uint64_t k2 = pack2(k, k);
+                times(v[i], Four{{k2, k2}, {k2, k2}});
+                times(v[i], load_weights<kHalf>(weights[h < q_heads ? 0 : 1], c16));
+            }
+            turn(v[i], turns);
+            float f[8];
+            in_order<kHalf>(v[i], f);
+            const uint2 lo = make_uint2(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]));
+            const uint2 hi = make_uint2(narrow2<DT>(f[4], f[5]), narrow2<DT>(f[6], f[7]));
+            uint16_t* to = h < q_heads ? yq + h * kDim : yk + (h - q_heads) * kDim;
+            if (row < rows) {
+                if (kHalf) {
+                    *reinterpret_cast<uint2*>(to + 4 * c16) = lo;
+                    *reinterpret_cast<uint2*>(to + 4 * c16 + 64) = hi;
+                } else {
+                    *reinterpret_cast<uint4*>(to + 8 * c16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                }
             }
         }
+    };
+    // (Every warp has four groups of copies, the last ones empty where it has fewer heads.  Lanes read what other lanes
+    // copied, hence the __syncwarp.)
+    wait_copies<3>();
+    __syncwarp();
+    group(0);
+    if (rows > 8) {
+        wait_copies<2>();
+        __syncwarp();
+        group(8);
+    }
+    if (rows > 16) {
+        wait_copies<1>();
+        __syncwarp();
+        group(16);
+    }
+    if (rows > 24) {
+        wait_copies<0>();
+        __syncwarp();
+        group(24);
     }
 }
 
 // The Q/K quantiser with the rotation in front: the turned values stay in float32 registers until their block's maximum
 // is known, so they are rounded once, to E4M3.  A CTA holds the angles of one block of 128 tokens in shared memory (64 KB)
-// and walks `rows_per_cta` heads of the list (heads of q, heads of k), 256 threads, eight tokens of sixteen bytes per thread,
-// the next head's loads issued before this head's maximum is reduced.  3 bytes per element (2 read, 1 written).
-template <int DT, bool kHalf>
-__global__ void __launch_bounds__(256, 2) rotary_quant_kernel(const __grid_constant__ RotaryArgs a, int blocks, int rows_per_cta) {
-    extern __shared__ __align__(16) float2 table[];  // [128][64]
-    __shared__ float part[2][8];
-    const int c16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-    const uint32_t lanes = 0xFFFFu << (threadIdx.x & 16);
+// and walks `rows_per_cta` heads of the list (heads of q, heads of k), 512 threads, four tokens of four pairs per thread,
+// the next head's loads issued before this head's maximum is reduced.  3 bytes per element (2 read, 1 written).  The norm's
+// factor of a row is not multiplied into its values but into the row's maximum and scale.
+constexpr int kQuantThreads = 512, kQuantRows = kTile * 16 / kQuantThreads, kQuantStep = kQuantThreads / 16;
+
+template <int DT, bool kHalf, bool kNorm>
+__global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __grid_constant__ RotaryArgs a, int blocks, int rows_per_cta) {
+    extern __shared__ __align__(16) float table[];  // cos [128][64], sin [128][64]
+    __shared__ uint32_t part[2][kQuantThreads / 32];
+    __shared__ Pairs pairs;
+    const int c16 = threadIdx.x & 15, r0 = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int blk = blockIdx.x;
     const long long b = blockIdx.z;
     const long long row0 = static_cast<long long>(blk) * kTile;
-    for (int i = threadIdx.x; i < kTile * kPairs; i += 256) {
-        const long long s = row0 + i / kPairs;
-        if (s < a.S) table[i] = pair_turn(a.angles, b * a.angles.batch_stride + s * a.angles.axes, i % kPairs);
-        else table[i] = make_float2(1.0f, 0.0f);
-    }
+    const int tokens = static_cast<int>(min(static_cast<long long>(kTile), a.S - row0));
     const int heads = a.src[0].heads;
     const int first = blockIdx.y * rows_per_cta, last = min(first + rows_per_cta, 2 * heads);
-    uint4 raw[8];
+    const long long block_at = (b * a.S + row0) * heads * kDim;  // inputs and codes are dense: elements before this block
+    const uint32_t pitch = static_cast<uint32_t>(heads) * kDim;  // elements from token to token; 128 tokens stay below 2^32
+    uint4 raw[kQuantRows];
     const auto load = [&](int row) {
-        const Source& t = a.src[row >= heads];
-        const uint16_t* x = t.x + b * t.batch + (row >= heads ? row - heads : row) * t.head + c16 * 8;
+        const uint16_t* x = (row >= heads ? a.src[1].x + (row - heads) * kDim : a.src[0].x + row * kDim) + block_at;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const long long s = row0 + r0 + 16 * i;
-            raw[i] = s < a.S ? ld_stream(x + s * t.token) : make_uint4(0, 0, 0, 0);
-        }
+        for (int i = 0; i < kQuantRows; ++i)
+            raw[i] = r0 + kQuantStep * i < tokens ? load_head<kHalf>(x + (r0 + kQuantStep * i) * pitch, c16) : make_uint4(0, 0, 0, 0);
     };
     load(first);
+    stage_pairs(a.angles, pairs);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kTile * kPairs; i += kQuantThreads) {
+        const long long s = row0 + min(i / kPairs, tokens - 1);
+        const float2 t = pair_turn(a.angles, pairs, b * a.angles.batch_stride + s * a.angles.axes, i % kPairs);
+        table[i] = t.x, table[kTile * kPairs + i] = t.y;
+    }
     __syncthreads();
     for (int row = first; row < last; ++row) {
         const Source& t = a.src[row >= heads];
         const int head = row >= heads ? row - heads : row;
-        float w[8];
-        if (t.weight != nullptr) {
+        Four v[kQuantRows];
+        float r[kQuantRows];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __ldg(t.weight + c16 * 8 + i);
-        }
-        float y[8][8], m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float2 cs[kHalf ? 8 : 4];
-            const float4* from = reinterpret_cast<const float4*>(table + (r0 + 16 * i) * kPairs + (kHalf ? 8 * (c16 & 7) : 4 * c16));
-#pragma unroll
-            for (int e = 0; e < (kHalf ? 4 : 2); ++e) {
-                const float4 two = from[e];
-                cs[2 * e] = make_float2(two.x, two.y), cs[2 * e + 1] = make_float2(two.z, two.w);
-            }
-            widen8<DT>(raw[i], y[i]);
-            norm_turn<kHalf>(y[i], t.weight != nullptr ? w : nullptr, a.angles.eps, cs, c16, lanes);
-            m = absmax8(y[i], m);
-        }
+        for (int i = 0; i < kQuantRows; ++i) v[i] = widen_pairs<DT, kHalf>(raw[i]);
         if (row + 1 < last) load(row + 1);
-        const float amax = fmaxf(cta256_max(m, part[row & 1]), kFloor);
+        const bool norm = kNorm && t.weight != nullptr;
+        if (norm) {
+            norm_factors<kQuantRows>(v, a.angles.eps, c16, r);
+            const Four w = load_weights<kHalf>(t.weight, c16);
+#pragma unroll
+            for (int i = 0; i < kQuantRows; ++i) times(v[i], w);
+        }
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kQuantRows; ++i) {
+            const float* from = table + (r0 + kQuantStep * i) * kPairs + 4 * c16;
+            turn(v[i], make_turns(*reinterpret_cast<const float4*>(from), *reinterpret_cast<const float4*>(from + kTile * kPairs)));
+            float f[8];
+            in_order<kHalf>(v[i], f);
+            float top = fmax3(fabsf(f[0]), fabsf(f[1]), fabsf(f[2]));
+            top = fmax3(top, fabsf(f[3]), fabsf(f[4]));
+            top = fmax3(top, fabsf(f[5]), fmaxf(fabsf(f[6]), fabsf(f[7])));
+            m = fmaxf(m, norm ? top * r[i] : top);
+        }
+        // (The order of non-negative floats is that of their bits.)
+        const uint32_t warp_top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+        if (lane == 0) part[row & 1][warp] = warp_top;
+        __syncthreads();
+        const float amax = fmaxf(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, part[row & 1][lane & (kQuantThreads / 32 - 1)])), kFloor);
         const float scale = div_full(kQMax, amax);
         if (threadIdx.x == 0) {
             float* descale = t.descale + (b * heads + head) * t.descale_stride;
@@ -216,11 +423,24 @@ __global__ void __launch_bounds__(256, 2) rotary_quant_kernel(const __grid_const
             if (blk == 0 && t.descale_stride > blocks) descale[blocks] = 1.0f;
             if (blk == 0 && row < heads && a.amax_init != nullptr) a.amax_init[b * heads + head] = 0.0f;
         }
-        uint8_t* dst = static_cast<uint8_t*>(t.y) + ((b * a.S + row0) * heads + head) * kDim + c16 * 8;
+        uint8_t* dst = static_cast<uint8_t*>(t.y) + block_at + head * kDim;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int r = r0 + 16 * i;
-            if (row0 + r < a.S) *reinterpret_cast<uint2*>(dst + static_cast<long long>(r) * heads * kDim) = quantize8(y[i], scale);
+        for (int i = 0; i < kQuantRows; ++i) {
+            const float k = norm ? scale * r[i] : scale;
+            const uint64_t k2 = pack2(k, k);
+            times(v[i], Four{{k2, k2}, {k2, k2}});
+            float f[8];
+            in_order<kHalf>(v[i], f);
+            const uint32_t lo = cast4(f[0], f[1], f[2], f[3]), hi = cast4(f[4], f[5], f[6], f[7]);  // (saturates at 448)
+            if (r0 + kQuantStep * i < tokens) {
+                uint8_t* to = dst + (r0 + kQuantStep * i) * pitch;
+                if (kHalf) {
+                    *reinterpret_cast<uint32_t*>(to + 4 * c16) = lo;
+                    *reinterpret_cast<uint32_t*>(to + 4 * c16 + 64) = hi;
+                } else {
+                    *reinterpret_cast<uint2*>(to + 8 * c16) = make_uint2(lo, hi);
+                }
+            }
         }
     }
 }
@@ -236,18 +456,30 @@ bool take_angles(const ovc_rotary* r, Angles* out) {
     out->type = r->position_type, out->axes = r->axes, out->eps = r->eps;
     for (int i = 0; i < kPairs; ++i) {
         if (!isfinite(r->turns[i]) || r->pair_axis[i] >= r->axes) return false;
-        out->turns[i] = r->turns[i], out->axis[i] = r->pair_axis[i];
+        const double fraction = r->turns[i] - floor(r->turns[i]);
+        out->turns[i] = fraction < 1.0 ? static_cast<unsigned long long>(ldexp(fraction, 64)) : 0;
+        out->axis[i] = r->pair_axis[i];
     }
     return true;
 }
 
 bool take_source(const void* x, void* y, const float* weight, const int64_t* strides, int64_t heads, uintptr_t out_mask, Source* out) {
-    if (!x || !y || !strides || !aligned16(x) || (reinterpret_cast<uintptr_t>(y) & out_mask) || (reinterpret_cast<uintptr_t>(weight) & 3u) ||
+    if (!x || !y || !strides || !aligned16(x) || (reinterpret_cast<uintptr_t>(y) & out_mask) || !aligned16(weight) ||
         strides[0] < 0 || strides[1] < 0 || strides[2] < 0 || strides[0] % 8 || strides[1] % 8 || strides[2] % 8)
         return false;
     out->x = static_cast<const uint16_t*>(x), out->y = y, out->weight = weight;
     out->batch = strides[0], out->token = strides[1], out->head = strides[2], out->heads = static_cast<int>(heads);
     return true;
+}
+
+// launch(bf16, half, norm) with the three as compile-time constants.
+template <class Launch>
+int by_variant(int dtype, const ovc_rotary* r, Launch launch) {
+    const auto norm = [&](auto bf16, auto half) {
+        return r->q_weight || r->k_weight ? launch(bf16, half, std::true_type{}) : launch(bf16, half, std::false_type{});
+    };
+    const auto half = [&](auto bf16) { return r->half_split ? norm(bf16, std::true_type{}) : norm(bf16, std::false_type{}); };
+    return dtype == OVC_BF16 ? half(std::true_type{}) : half(std::false_type{});
 }
 
 bool bad_shape(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk) {
@@ -268,21 +500,22 @@ extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void
         !take_source(k, k_out, rotary->k_weight, k_strides, Hk, 15, &a.src[1]))
         return OVC_ERR_ARGUMENT;
     a.S = S, a.tokens = B * S;
-    // As many tokens per CTA (up to sixteen) as leave a few CTAs per SM, more where a token has fewer heads than the CTA's
-    // half warps; with one token per CTA and still too few CTAs, the heads are split.
-    const int rows = static_cast<int>(Hq + Hk);
-    int tile = 16;
-    while (tile > 1 && (ceil_div(a.tokens, tile) < 4 * 148 && 16 / tile < rows)) tile /= 2;
-    int splits = 1;
-    while (ceil_div(a.tokens, tile) * splits < 2 * 148 && splits * (16 / tile) < rows) ++splits;
-    const int per_cta = static_cast<int>(ceil_div(rows, splits));
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, tile)), static_cast<unsigned>(ceil_div(rows, per_cta)));
+    // A warp takes up to 32 heads, fewer where that would leave SMs without a few warps each.
+    const int64_t rows = Hq + Hk, share = a.tokens * rows / (8 * 148);
+    int64_t unit_rows = share > kUnitRows ? kUnitRows : share < 2 ? 2 : share;
+    const int64_t units = ceil_div(rows, unit_rows);
+    unit_rows = ceil_div(ceil_div(rows, units), 2) * 2;
+    const int64_t ctas = ceil_div(a.tokens * units, kUnitWarps);
+    if (ctas > 0x7FFFFFFF) return OVC_ERR_ARGUMENT;
+    const unsigned grid = static_cast<unsigned>(ctas);
+    const size_t smem = static_cast<size_t>(kUnitWarps * unit_rows * 256);
     auto s = static_cast<cudaStream_t>(stream);
-    if (dtype == OVC_BF16 && rotary->half_split) rotary_kernel<OVC_BF16, true><<<grid, 256, 0, s>>>(a, tile, per_cta);
-    else if (dtype == OVC_BF16) rotary_kernel<OVC_BF16, false><<<grid, 256, 0, s>>>(a, tile, per_cta);
-    else if (rotary->half_split) rotary_kernel<OVC_F16, true><<<grid, 256, 0, s>>>(a, tile, per_cta);
-    else rotary_kernel<OVC_F16, false><<<grid, 256, 0, s>>>(a, tile, per_cta);
-    return check_launch();
+    const auto launch = [&](auto bf16, auto half, auto norm) {
+        rotary_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>
+            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(unit_rows), static_cast<int>(units));
+        return check_launch();
+    };
+    return by_variant(dtype, rotary, launch);
 }
 
 namespace {
@@ -298,28 +531,37 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     a.S = S, a.tokens = B * S, a.amax_init = amax_init;
     a.src[0].descale = q_descale, a.src[0].descale_stride = q_stride;
     a.src[1].descale = k_descale, a.src[1].descale_stride = k_stride;
-    // A CTA computes its block's angles once, so it takes as many heads as leave a few CTAs per SM.
+    // Two CTAs run per SM.  Heads per CTA: the count whose rounds of CTAs, each of its heads and the block's angles (which
+    // cost about as much as two heads), are the shortest in all.
     const int rows = static_cast<int>(2 * H);
-    const int64_t splits = ceil_div(4 * 2 * 148, blocks * B);
-    const int per_cta = static_cast<int>(splits >= rows ? 1 : ceil_div(rows, splits));
+    int per_cta = 1;
+    int64_t best = 0;
+    for (int n = 1; n <= rows; ++n) {
+        const int64_t cost = ceil_div(blocks * B * ceil_div(rows, n), 2 * 148) * (n + 2);
+        if (n == 1 || cost <= best) best = cost, per_cta = n;
+    }
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(rows, per_cta)), static_cast<unsigned>(B));
     constexpr int smem = kTile * kPairs * static_cast<int>(sizeof(float2));
     auto s = static_cast<cudaStream_t>(stream);
-    const auto launch = [&](auto kernel) {
+    const auto launch = [&](auto bf16, auto half, auto norm) {
+        const auto kernel = rotary_quant_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>;
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (err != cudaSuccess) { set_last_cuda_error(err); return static_cast<int>(OVC_ERR_CUDA); }
-        kernel<<<grid, 256, smem, s>>>(a, static_cast<int>(blocks), per_cta);
+        kernel<<<grid, kQuantThreads, smem, s>>>(a, static_cast<int>(blocks), per_cta);
         return check_launch();
     };
-    if (dtype == OVC_BF16) return rotary->half_split ? launch(rotary_quant_kernel<OVC_BF16, true>) : launch(rotary_quant_kernel<OVC_BF16, false>);
-    return rotary->half_split ? launch(rotary_quant_kernel<OVC_F16, true>) : launch(rotary_quant_kernel<OVC_F16, false>);
+    return by_variant(dtype, rotary, launch);
 }
 
 }  // namespace
 
-extern "C" int ovc_quantize_qk_rotary(const void* q, const void* k, int dtype, int64_t B, int64_t S, int64_t H, const ovc_rotary* rotary,
-                                      void* q8, void* k8, float* q_descale, int64_t q_stride, float* k_descale, int64_t k_stride, void* stream) {
-    return launch_rotary_quant(q, k, dtype, B, S, H, rotary, q8, k8, q_descale, q_stride, k_descale, k_stride, nullptr, stream);
+extern "C" int ovc_prepare_rotary(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t S, int64_t H,
+                                  const ovc_rotary* rotary, void* q8, void* k8, void* v8, float* q_descale, float* k_descale,
+                                  float* v_descale, float* amax_ws, void* stream) {
+    if (!v || !v8 || !v_descale || !amax_ws || !aligned16(v) || (reinterpret_cast<uintptr_t>(v8) & 7u)) return OVC_ERR_ARGUMENT;
+    const int64_t blocks = ceil_div(S, kTile);
+    const int rc = launch_rotary_quant(q, k, dtype, B, S, H, rotary, q8, k8, q_descale, blocks, k_descale, blocks, amax_ws, stream);
+    return rc != OVC_OK ? rc : launch_amax_cast_v(v, dtype, B, S, H, amax_ws, v8, v_descale, stream);
 }
 
 extern "C" int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H, const ovc_rotary* rotary,

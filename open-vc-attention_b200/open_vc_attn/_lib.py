@@ -48,7 +48,7 @@ SIGNATURES = {
     "ovc_attention_packed": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _l, _l, _l, _l, _l, _i, _f, _p, _p, _p, _p, _p, _p]),
     "ovc_attention_packed_workspace": (_l, [_l, _l, _l, _l, _l]),
     "ovc_rotary_qk": (_i, [_p, _p, _p, _p, _i, _l, _l, _l, _l, _p, _p, _p, _p]),
-    "ovc_quantize_qk_rotary": (_i, [_p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _l, _p, _l, _p]),
+    "ovc_prepare_rotary": (_i, [_p, _p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "ovc_prepare_fused_rotary": (_i, [_p, _p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "ovc_vs_assign": (_i, [_p, _p, _p, _l, _l, _l, _p]),
     "ovc_vs_accumulate": (_i, [_p, _p, _p, _p, _l, _l, _l, _p]),
@@ -101,3 +101,29 @@ def stream_pointer(device):
     import torch
 
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def raw_stream(index):
+    """The current stream of device ``index`` as stream_pointer gives it, without making a Stream object (2 us less a call)."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+class on_device:
+    """Makes ``device`` current for a with block; costs nothing where it is current already."""
+
+    __slots__ = ("guard",)
+
+    def __init__(self, device):
+        import torch
+
+        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exception):
+        if self.guard is not None:
+            self.guard.__exit__(*exception)

@@ -51,10 +51,11 @@ def _layout(q, k, v):
     if q.ndim == 3 or q.shape[0] == 1:
         q, k, v = [t.reshape(-1, t.shape[-2], t.shape[-1]).contiguous() for t in (q, k, v)]
         sq, sk = q.shape[0], k.shape[0]
+        # [0, S], built on the device (one launch) so that the call stays capturable in a CUDA graph.
+        cu_q = torch.arange(0, sq + 1, sq, device=q.device, dtype=torch.int32)
         kwargs = {
-            # Built on the device so that the call stays capturable in a CUDA graph.
-            "cu_seqlens_q": torch.arange(2, device=q.device, dtype=torch.int32) * sq,
-            "cu_seqlens_k": torch.arange(2, device=q.device, dtype=torch.int32) * sk,
+            "cu_seqlens_q": cu_q,
+            "cu_seqlens_k": cu_q if sk == sq else torch.arange(0, sk + 1, sk, device=q.device, dtype=torch.int32),
             "max_seqlen_q": sq,
             "max_seqlen_k": sk,
         }
@@ -118,12 +119,12 @@ def prepare_fp8(q, k, v, *, rotary=None):
     with torch.cuda.device(q.device):
         q, k, v, layout, shape = _layout(q, k, v)
         if rotary is not None:
-            from .rotary import quantize_qk
+            from .rotary import prepare_rotary
 
-            q8, qs, k8, ks = quantize_qk(q, k, rotary)
-        else:
-            q8, qs = fp8_quantize_per_block(q, block_l=128)
-            k8, ks = fp8_quantize_per_block(k, block_l=128)
+            codes, descales = prepare_rotary(q, k, v, rotary)
+            return PreparedFP8(*codes, *descales, layout, shape)
+        q8, qs = fp8_quantize_per_block(q, block_l=128)
+        k8, ks = fp8_quantize_per_block(k, block_l=128)
         v8, vs = fp8_quantize_per_head(v)
         if q.ndim == 3:
             q8, k8, v8 = q8[0], k8[0], v8[0]

@@ -7,6 +7,7 @@ those functions use: FP8 E4M3 Q/K/V with FP32 descales, ExpCast, optional causal
 optional prepacked V and optional repair prefix.  Anything else raises instead of degrading.
 """
 
+import ctypes
 import math
 
 import torch
@@ -14,6 +15,7 @@ import torch
 from . import _lib
 
 _status_words = {}
+_mirrored = {}  # the mirrors' memory, for reading one without a tensor operation
 
 
 def status_word(device):
@@ -30,6 +32,7 @@ def _status(device):
         words = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", key))
         mirror = torch.zeros(1, dtype=torch.int32).pin_memory()  # host copy of words[1], refreshed after every launch
         _status_words[key] = (words, mirror)
+        _mirrored[key] = ctypes.c_int32.from_address(mirror.data_ptr())
     return _status_words[key]
 
 
@@ -43,6 +46,9 @@ def _failure(value):
 def _raise_if_flagged(device):
     """No synchronisation: looks at the host copy of the sticky word, which reflects every launch whose
     trailing 4-byte copy has completed.  Called at the start of each public attention call."""
+    flag = _mirrored.get(device.index)
+    if flag is not None and flag.value == 0:
+        return
     words, mirror = _status(device)
     value = int(mirror[0])
     if value != 0:

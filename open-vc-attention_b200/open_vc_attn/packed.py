@@ -12,6 +12,7 @@ import math
 import torch
 
 from . import _lib
+from .forward import _raise_if_flagged, _status
 
 
 def _strides(t):
@@ -87,13 +88,11 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
         flags |= _lib.OVC_ATTN_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of Q's shape, type and device")
-    from .forward import _raise_if_flagged, _status
-
     lib = _lib.load()
     _raise_if_flagged(device)
-    with torch.cuda.device(device):
+    with _lib.on_device(device):
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty((hq, tq), dtype=torch.float32, device=device) if return_lse else None
         if tq == 0:
             return (out, lse) if return_lse else out
@@ -122,7 +121,7 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
                 *arguments, _lib.dtype_code(q.dtype), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *sizes, flags,
                 softmax_scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
                 None if workspace is None else workspace.data_ptr(), words.data_ptr() + 4, mirror.data_ptr(),
-                _lib.stream_pointer(device),
+                _lib.raw_stream(device.index),
             ),
             "ovc_attention_packed",
         )

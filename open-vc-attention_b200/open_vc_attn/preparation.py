@@ -4,8 +4,6 @@ Host side of ovc_prepare_fused; mirrors prepare_fp8_fused of the reference
 (src/open_vc_attn/preparation.py:83-162): same validation and messages, same result layout.
 """
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -51,7 +49,7 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
     lib = _lib.load()
     with torch.cuda.device(q.device):
         if cu_seqlens is None:
-            cu_seqlens = torch.arange(2, device=q.device, dtype=torch.int32) * s
+            cu_seqlens = torch.arange(0, s + 1, s, device=q.device, dtype=torch.int32)
         blocks = (s + 127) // 128
         q_blocks = (blocks + 1) // 2 * 2
         padded = blocks * 128
@@ -66,7 +64,7 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
         if rotary is None:
             _lib.check(lib.ovc_prepare_fused(*inputs, *outputs), "ovc_prepare_fused")
         else:
-            _lib.check(lib.ovc_prepare_fused_rotary(*inputs, ctypes.byref(rotary.arguments), *outputs), "ovc_prepare_fused_rotary")
+            _lib.check(lib.ovc_prepare_fused_rotary(*inputs, rotary.arguments, *outputs), "ovc_prepare_fused_rotary")
         result = packed[..., :s].movedim(-1, 0)
         layout = dict(cu_seqlens_q=cu_seqlens, cu_seqlens_k=cu_seqlens, max_seqlen_q=s, max_seqlen_k=s)
         return PreparedFP8(q8, k8, result, qs, ks, vs, layout, shape, v_prepacked=True)

@@ -28,9 +28,9 @@ class RotaryPlan:
     q_weight: torch.Tensor
     k_weight: torch.Tensor
     eps: float
-    turns: tuple
-    pair_axis: tuple
-    arguments: object  # the C struct; points into the tensors above
+    turns: object
+    pair_axis: object
+    arguments: object  # a pointer to the C struct, which points into the members above
 
     def check(self, q, k, name="rotary"):
         """Raise unless the plan fits Q and K ([S,H,128] or [B,S,H,128])."""
@@ -42,8 +42,9 @@ class RotaryPlan:
             raise ValueError("Rotary positions need Q and K of the same tokens")
         if self.positions.device != q.device:
             raise ValueError("Rotary positions must reside with Q and K")
-        if tuple(self.positions.shape[:-1]) not in ((s,), (batch, s)):
-            raise ValueError(f"Rotary positions are for {tuple(self.positions.shape[:-1])} tokens, Q and K have {(batch, s)}")
+        tokens = self.positions.shape[:-1]
+        if tokens != (s,) and tokens != (batch, s):
+            raise ValueError(f"Rotary positions are for {tuple(tokens)} tokens, Q and K have {(batch, s)}")
 
 
 def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True, frequencies="axis", q_weight=None,
@@ -88,6 +89,7 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
             if tuple(w.shape) != (128,) or not w.is_floating_point() or w.device != positions.device:
                 raise ValueError(f"{name} must be a floating-point tensor of 128 values with the positions")
             w = w.detach().float().contiguous()
+            w = w.clone() if w.data_ptr() % 16 else w
         weights.append(w)
     pair_axis = [a for a, d in enumerate(axes) for _ in range(d // 2)]
     if frequencies == "axis":
@@ -104,7 +106,7 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
         ctypes.addressof(host[1]), *[None if w is None else w.data_ptr() for w in weights], _POSITION_TYPES[positions.dtype],
         len(axes), 0 if interleaved else 1, eps,
     )
-    return RotaryPlan(positions, axes, bool(interleaved), *weights, float(eps), host[0], host[1], arguments)
+    return RotaryPlan(positions, axes, bool(interleaved), *weights, float(eps), *host, ctypes.pointer(arguments))
 
 
 def grid_positions(frames, height, width, *, text=0, start=(0, 0, 0), device="cuda"):
@@ -117,23 +119,29 @@ def grid_positions(frames, height, width, *, text=0, start=(0, 0, 0), device="cu
     return torch.cat([clip.new_zeros((text, 3)), clip]) if text else clip
 
 
-def readable(t):
-    """``t`` itself where its heads can be read in place by 16-byte accesses, else a dense copy."""
-    strides = t.stride()
-    if strides[-1] == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides[:-1]):
-        return t
-    return t.contiguous()
+def _strides(t):
+    """Elements from one batch item, token and head of [S,H,128] or [B,S,H,128] to the next; None where the heads cannot be
+    read in place by 16-byte accesses."""
+    stride, shape = t.stride(), t.shape
+    if stride[-1] != 1 or t.data_ptr() % 16:
+        return None
+    # the stride of a dimension of one entry is never used, and may be anything
+    used = [0 if n == 1 else s for n, s in zip(shape[:-1], stride)]
+    if any(s % 8 for s in used):
+        return None
+    return used if len(used) == 3 else [0, *used]
 
 
 def rotary_qk(q, k, plan):
     """Rotated (and, with weights, normalised) Q and K, in new dense tensors of their types.
 
     q [S,Hq,128] or [B,S,Hq,128], k with the same tokens and any number of heads, float16 or bfloat16.  Slices of a fused
-    projection are read in place.  float32 inside (angles in float64), rounded once.
+    projection are read in place.  float32 inside (angles in 64-bit fixed point), rounded once.
     """
     if q.ndim not in (3, 4) or k.ndim != q.ndim or q.shape[-1] != 128 or k.shape[-1] != 128 or min(q.shape[-2], k.shape[-2]) < 1:
         raise ValueError("Expected [S,H,128] or [B,S,H,128] Q/K")
-    if not q.is_cuda or k.device != q.device:
+    device = q.device
+    if not q.is_cuda or k.device != device:
         raise ValueError("Q/K must reside on the same CUDA device")
     if q.requires_grad or k.requires_grad:
         raise ValueError("Forward inference only; detach inputs explicitly")
@@ -142,36 +150,45 @@ def rotary_qk(q, k, plan):
     code = _lib.dtype_code(q.dtype)
     RotaryPlan.check(plan, q, k, "plan")
     lib = _lib.load()
-    with torch.cuda.device(q.device):
-        q_out, k_out = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
+    with _lib.on_device(device):
+        outs, arguments, keep = [], [], []
+        for t in (q, k):
+            outs.append(torch.empty_like(t, memory_format=torch.contiguous_format))
+            strides = _strides(t)
+            if strides is None:
+                t = t.clone(memory_format=torch.contiguous_format)
+                strides = [t.shape[-3] * t.shape[-2] * 128, t.shape[-2] * 128, 128]
+            keep.append(t)
+            arguments += [t.data_ptr(), (ctypes.c_int64 * 3)(*strides)]
         if q.numel() == 0:
-            return q_out, k_out
-        q, k = readable(q), readable(k)
-        batch = q.shape[0] if q.ndim == 4 else 1
-        strides = [(ctypes.c_int64 * 3)(*((0,) * (4 - t.ndim) + t.stride()[:-1])) for t in (q, k)]
+            return tuple(outs)
         _lib.check(
             lib.ovc_rotary_qk(
-                q.data_ptr(), strides[0], k.data_ptr(), strides[1], code, batch, q.shape[-3], q.shape[-2], k.shape[-2],
-                ctypes.byref(plan.arguments), q_out.data_ptr(), k_out.data_ptr(), _lib.stream_pointer(q.device),
+                *arguments, code, q.shape[0] if q.ndim == 4 else 1, q.shape[-3], q.shape[-2], k.shape[-2], plan.arguments,
+                outs[0].data_ptr(), outs[1].data_ptr(), _lib.raw_stream(device.index),
             ),
             "ovc_rotary_qk",
         )
-    return q_out, k_out
+    return tuple(outs)
 
 
-def quantize_qk(q, k, plan):
-    """fp8_quantize_per_block of rotated Q and K: (q codes, q descale, k codes, k descale), one launch."""
+def prepare_rotary(q, k, v, plan):
+    """fp8_quantize_per_block of rotated Q and K and fp8_quantize_per_head of V, dense inputs: codes of the inputs' shapes, and
+    (q, k, v) descales [B,H,blocks], [B,H,blocks], [B,H]."""
     batch = q.shape[0] if q.ndim == 4 else 1
-    s, h = q.shape[-3:-1]
+    s, h, _ = q.shape[-3:]
     blocks = (s + 127) // 128
-    lib = _lib.load()
-    q8, k8 = [torch.empty((batch, s, h, 128), dtype=torch.float8_e4m3fn, device=q.device) for _ in range(2)]
-    qs, ks = [torch.empty((batch, h, blocks), dtype=torch.float32, device=q.device) for _ in range(2)]
+    codes = [torch.empty_like(t, dtype=torch.float8_e4m3fn) for t in (q, k, v)]
+    qs = torch.empty((batch, h, blocks), dtype=torch.float32, device=q.device)
+    ks = torch.empty_like(qs)
+    vs = torch.empty((batch, h), dtype=torch.float32, device=q.device)
+    amax = torch.empty_like(vs)
     _lib.check(
-        lib.ovc_quantize_qk_rotary(
-            q.data_ptr(), k.data_ptr(), _lib.dtype_code(q.dtype), batch, s, h, ctypes.byref(plan.arguments), q8.data_ptr(),
-            k8.data_ptr(), qs.data_ptr(), blocks, ks.data_ptr(), blocks, _lib.stream_pointer(q.device),
+        _lib.load().ovc_prepare_rotary(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), batch, s, h, plan.arguments,
+            *[t.data_ptr() for t in codes], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), amax.data_ptr(),
+            _lib.raw_stream(q.device.index),
         ),
-        "ovc_quantize_qk_rotary",
+        "ovc_prepare_rotary",
     )
-    return q8, qs, k8, ks
+    return codes, (qs, ks, vs)

@@ -84,10 +84,12 @@ def test_c_entries_refuse_bad_arguments():
     turns[3] = float("inf")
     assert rotate() == bad
     turns[3] = 0.0
-    quant = lib.ovc_quantize_qk_rotary
-    assert quant(p, p, 1, 1, 300, 1, plan(), p, p, p, 2, p, 3, None) == bad      # descale row too short
-    assert quant(p, p, 1, 1, 128, 1, plan(), p + 4, p, p, 1, p, 1, None) == bad  # misaligned codes
-    assert quant(p, p, 7, 1, 128, 1, plan(), p, p, p, 1, p, 1, None) == bad
+    general = lib.ovc_prepare_rotary
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p + 4, p, p, p, p, p, p, None) == bad  # misaligned codes
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p + 4, p, p, p, p, None) == bad
+    assert general(p, p, p, 7, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p, p, None, p, p, None) == bad
+    assert general(p, p, p + 2, 1, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
     fused = lib.ovc_prepare_fused_rotary
     assert fused(p, p, None, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
     assert fused(p, p, p, 1, 128, 1, None, p, p, p, p, p, p, p, None) == bad
