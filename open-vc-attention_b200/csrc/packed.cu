@@ -212,38 +212,37 @@ __host__ __device__ constexpr uint32_t idesc(bool b_mn_major) {
            (static_cast<uint32_t>(kTile >> 3) << 17) | (static_cast<uint32_t>(kTile >> 4) << 24);
 }
 
-__device__ __forceinline__ uint64_t desc(uint32_t lo) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(kSmemDescHi));
-    return d;
-}
-
-// S = Q K^T: both operands K-major, 64 channels to a half; eight steps of 16 channels (32 bytes).  One thread.
+// The products are issued by one elected lane while the whole warp executes the (convergent) code, so that descriptors and
+// addresses are warp-uniform values and need no moves between the products.
+// S = Q K^T: both operands K-major, 64 channels to a half; eight steps of 16 channels (32 bytes).
 __device__ __forceinline__ void product_qk(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t id) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t step = (k >> 2) * (kHalfBytes >> 4) + (k & 3) * 2;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "l"(desc(a_lo + step)), "l"(desc(b_lo + step)), "r"(id), "r"(k)
-            : "memory");
-    }
+#define OVC_QK_STEP(offset, accumulate)                                                                  \
+    "add.u32 al, %1, " #offset ";\n\tadd.u32 bl, %2, " #offset ";\n\tmov.b64 da, {al, %3};\n\tmov.b64 db, {bl, %3};\n\t" \
+    "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, " #accumulate ";\n\t"
+    static_assert((kHalfBytes >> 4) == 1024, "the second half's offset is written out below");
+    asm volatile(
+        "{\n\t.reg .pred leader;\n\t.reg .b64 da, db;\n\t.reg .b32 al, bl;\n\t"
+        "elect.sync _|leader, 0xFFFFFFFF;\n\t"
+        OVC_QK_STEP(0, 0) OVC_QK_STEP(2, 1) OVC_QK_STEP(4, 1) OVC_QK_STEP(6, 1)
+        OVC_QK_STEP(1024, 1) OVC_QK_STEP(1026, 1) OVC_QK_STEP(1028, 1) OVC_QK_STEP(1030, 1) "}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(kSmemDescHi), "r"(id)
+        : "memory");
+#undef OVC_QK_STEP
 }
 // O (+)= P V: P in tensor memory (two values per column), V as the MN-major operand (a row of shared memory is a key);
-// eight steps of 16 keys.  One thread.
-__device__ __forceinline__ void product_pv(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t id, bool accumulate) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-            ::"r"(d_tmem), "r"(a_tmem + 8 * k), "l"(desc(b_lo + 128 * k)), "r"(id), "r"(k > 0 || accumulate ? 1 : 0)
-            : "memory");
-    }
-}
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// four steps of 16 keys, a half of a tile.
+__device__ __forceinline__ void product_pv(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t id, uint32_t accumulate_first) {
+#define OVC_PV_STEP(a_offset, b_offset, accumulate)                                                      \
+    "add.u32 ta, %1, " #a_offset ";\n\tadd.u32 bl, %2, " #b_offset ";\n\tmov.b64 db, {bl, %3};\n\t"      \
+    "@leader tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], db, %4, " accumulate ";\n\t"
+    asm volatile(
+        "{\n\t.reg .pred leader, p;\n\t.reg .b64 db;\n\t.reg .b32 ta, bl;\n\t"
+        "elect.sync _|leader, 0xFFFFFFFF;\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        OVC_PV_STEP(0, 0, "p") OVC_PV_STEP(8, 128, "1") OVC_PV_STEP(16, 256, "1") OVC_PV_STEP(24, 384, "1") "}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(kSmemDescHi), "r"(id), "r"(accumulate_first)
+        : "memory");
+#undef OVC_PV_STEP
 }
 
 template <bool kBf16>
@@ -263,13 +262,36 @@ __device__ __forceinline__ void unpack2(uint64_t v, float* a, float* b) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
 }
 
+// Row maximum that is not a number where a score is not.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max128_nan(const uint32_t (&s)[128]) {
+    const auto v = [&](int i) { return __uint_as_float(s[i]); };
+    float m[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        float a[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a[i] = fmax3_nan(v(32 * c + i), v(32 * c + 8 + i), v(32 * c + 16 + i));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = fmax3_nan(a[i], a[i + 4], v(32 * c + 24 + i));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) a[i] = fmax3_nan(a[i], a[i + 2], v(32 * c + 28 + i));
+        m[c] = fmax3_nan(a[0], a[1], fmax3_nan(v(32 * c + 30), v(32 * c + 31), v(32 * c + 31)));
+    }
+    return fmax3_nan(fmax3_nan(m[0], m[1], m[2]), m[3], m[3]);
+}
+
 struct Smem {
     alignas(1024) uint8_t q[2][kTileBytes];
     alignas(1024) uint8_t ring[kSlots][kTileBytes];
     alignas(8) uint64_t q_full[2];
     uint64_t full[kSlots], empty[kSlots];  // a tile has landed / its last reader is done
     uint64_t s_full[2];                    // the stage's scores are in tensor memory
-    uint64_t p_full[2];                    // the stage's probabilities are, and O is rescaled
+    uint64_t p_full[2][2];                 // the stage's probabilities of the first, second 64 keys are, and O is rescaled
     uint64_t o_full[2];
     uint64_t v_clean;                      // the rows behind the sequence's end are cleared in its last value tile
     uint64_t drain;
@@ -342,7 +364,8 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             for (int i = 0; i < 2; ++i) {
                 mbar_init(smem_addr(&sm.q_full[i]), 1);
                 mbar_init(smem_addr(&sm.s_full[i]), 1);
-                mbar_init(smem_addr(&sm.p_full[i]), 128);
+                mbar_init(smem_addr(&sm.p_full[i][0]), 128);
+                mbar_init(smem_addr(&sm.p_full[i][1]), 128);
                 mbar_init(smem_addr(&sm.o_full[i]), 1);
             }
             for (int i = 0; i < kSlots; ++i) {
@@ -417,40 +440,77 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 for (int s = 0; s < q_tiles; ++s)
                     while (!mbar_try_wait(smem_addr(&sm.q_full[s]), 0) && clock64() - t0 < kWaitCycles) {}
             }
-        } else if (warp == 9 && lane == 0 && run) {
+        } else if (warp == 9 && run) {
             // ---------------- products ----------------
+            // One warp issues for both stages, in a fixed order, which keeps them half a step apart (with a warp for each
+            // stage they drifted into step: 1.25 times the time).  The issuing lane is held until all but the last
+            // products have run, so what lies between two issues is kept short: slots and descriptors are carried along,
+            // the copies are waited for by the first stage that needs them (in the narrow form, where keys are what is
+            // waited for, K of the next step only once V's slot is on its way back).
             constexpr uint32_t id_qk = idesc<kBf16>(false), id_pv = idesc<kBf16>(true);
-            const auto landed = [&](int index) { return wait(&sm.full[index % kSlots], (index / kSlots) & 1); };
-            const auto scores = [&](int s, int n) {
-                const int index = 2 * tile_of<kMode>(s, n);
-                if (!landed(index)) return false;
-                product_qk(tmem + kColS + 128 * s, smem_desc_lo(smem_addr(sm.q[kMode == kSplitNarrow ? 0 : s])),
-                           smem_desc_lo(smem_addr(sm.ring[index % kSlots])), id_qk);
-                commit(&sm.s_full[s]);
-                if (kMode == kSplitNarrow || s == 1 || n >= steps[1]) commit(&sm.empty[index % kSlots]);
-                return true;
+            const auto uniform = [](int x) { return static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(x))); };
+            const int steps0 = uniform(steps[0]), steps1 = uniform(steps[1]), dirty = uniform(cleans ? n_tiles : 0) - 1;
+            const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
+            const auto all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)) != 0; };
+            struct Slot {
+                int i = 0;
+                uint32_t phase = 0;
+                __device__ __forceinline__ void advance() { if (++i == kSlots) i = 0, phase ^= 1; }
             };
+            const uint32_t ring_lo = smem_desc_lo(smem_addr(sm.ring[0])), q_lo = smem_desc_lo(smem_addr(sm.q[0]));
+            const uint32_t ring_lo_mn = smem_desc_lo_bmn(smem_addr(sm.ring[0]), kHalfBytes);
+            const auto scores = [&](int s, const Slot& k, bool last_reader) {
+                product_qk(tm + kColS + 128 * s, q_lo + (kMode == kSplitNarrow ? 0 : s * (kTileBytes >> 4)), ring_lo + k.i * (kTileBytes >> 4), id_qk);
+                mma_commit_elect(smem_addr(&sm.s_full[s]));
+                if (last_reader) mma_commit_elect(smem_addr(&sm.empty[k.i]));
+            };
+            // Slots of K of a stage's next step and V of its present one.
+            Slot k, v;
+            v.advance();
             bool ok = true;
-            for (int s = 0; ok && s < 2; ++s)
-                if (steps[s] > 0) ok = wait(&sm.q_full[kMode == kSplitNarrow ? 0 : s], 0) && scores(s, 0);
-            const int most = max(steps[0], steps[1]);
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (ok && (s ? steps1 : steps0) > 0) {
+                    ok = all(&sm.q_full[kMode == kSplitNarrow ? 0 : s], 0) && all(&sm.full[k.i], k.phase);
+                    if (ok) scores(s, k, kMode == kSplitNarrow || s == 1 || steps1 == 0);
+                }
+                if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance();
+            }
+            const int most = max(steps0, steps1);
             for (int n = 0; ok && n < most; ++n) {
-                for (int s = 0; ok && s < 2; ++s) {
-                    if (n >= steps[s]) continue;
-                    const int index = 2 * tile_of<kMode>(s, n) + 1;
-                    ok = landed(index) && (!cleans || tile_of<kMode>(s, n) != n_tiles - 1 || wait(&sm.v_clean, 0)) &&
-                         wait(&sm.p_full[s], n & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    product_pv(tmem + kColO + 128 * s, tmem + kColS + 128 * s,
-                               smem_desc_lo_bmn(smem_addr(sm.ring[index % kSlots]), kHalfBytes), id_pv, n > 0);
-                    if (n + 1 == steps[s]) commit(&sm.o_full[s]);
-                    if (kMode == kSplitNarrow || s == 1 || n >= steps[1]) commit(&sm.empty[index % kSlots]);
-                    if (n + 1 < steps[s]) ok = scores(s, n + 1);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const int mine = s ? steps1 : steps0;
+                    if (n < mine) {
+                        const uint32_t t_o = tm + kColO + 128 * s, t_p = tm + kColS + 128 * s, v_lo = ring_lo_mn + v.i * (kTileBytes >> 4);
+                        const bool first = kMode == kSplitNarrow || s == 0 || n >= steps0, last = kMode == kSplitNarrow || s == 1 || n >= steps1;
+                        const bool more = n + 1 < mine;
+                        if (first) {
+                            ok = all(&sm.full[v.i], v.phase) && (tile_of<kMode>(s, n) != dirty || all(&sm.v_clean, 0));
+                            if (kMode != kSplitNarrow && more) ok = ok && all(&sm.full[k.i], k.phase);
+                        } else if (more && n + 1 >= steps0) {
+                            ok = all(&sm.full[k.i], k.phase);
+                        }
+                        // The first half of the keys is multiplied while the stage still works on the second.
+                        ok = ok && all(&sm.p_full[s][0], n & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        product_pv(t_o, t_p, v_lo, id_pv, n > 0);
+                        ok = all(&sm.p_full[s][1], n & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        product_pv(t_o, t_p + 32, v_lo + 512, id_pv, 1);
+                        if (last) mma_commit_elect(smem_addr(&sm.empty[v.i]));
+                        if (kMode == kSplitNarrow && more) ok = all(&sm.full[k.i], k.phase);
+                        if (!ok) break;
+                        if (more) scores(s, k, kMode == kSplitNarrow || s == 1 || n + 1 >= steps1);
+                        else mma_commit_elect(smem_addr(&sm.o_full[s]));
+                    }
+                    if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance(), v.advance(), v.advance();
                 }
             }
             if (!ok) {  // products in flight end before tensor memory is released
-                commit(&sm.drain);
+                mma_commit_elect(smem_addr(&sm.drain));
                 const long long t0 = clock64();
                 while (!mbar_try_wait(smem_addr(&sm.drain), 0) && clock64() - t0 < kWaitCycles) {}
             }
@@ -472,6 +532,10 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 
         float top = -INFINITY;     // the maximum that the accumulator is scaled by
         float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
+        float limit = -INFINITY;   // a scaled score above it moves the maximum
+        // Steps whose tile every row of the warp sees in full.
+        const int whole_tiles = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(keys))) / kTile - item.t0;
+        const int whole_steps = kMode == kSplitNarrow ? (whole_tiles - stage + 1) / 2 : whole_tiles;
         uint64_t sum2 = 0;         // the running sum, even and odd columns
         bool ok = true;
         for (int n = 0; n < my_steps; ++n) {
@@ -484,53 +548,62 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             tmem_ld32(t_s + 64, s + 64);
             tmem_ld32(t_s + 96, s + 96);
             tmem_wait_ld();
-            const int columns = keys - (item.t0 + tile_of<kMode>(stage, n)) * kTile;
-            if (__any_sync(0xFFFFFFFFu, columns < kTile)) {
+            if (n >= whole_steps) {
+                const int columns = keys - (item.t0 + tile_of<kMode>(stage, n)) * kTile;
 #pragma unroll
                 for (int c = 0; c < 128; ++c)
                     if (c >= columns) s[c] = 0xFF800000u;  // -inf, whatever the key holds
             }
             // The maximum moves only when it grows by more than 2^8: until then probabilities above 1 are as exact as those
-            // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.
-            const float tile_top = max128(s);
-            float alpha = 1.0f;
-            if ((tile_top - top) * p.scale_log2 > 8.0f) {  // also the first finite maximum: top is -inf
-                alpha = ex2(fmaf(top, p.scale_log2, -tile_top * p.scale_log2));
-                top = tile_top;
-                shift = -top * p.scale_log2;
+            // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.  The
+            // comparison is false where both are -inf (no key yet) and true where a score is not a number.
+            const float tile_top = max128_nan(s);
+            if (__any_sync(0xFFFFFFFFu, !(tile_top * p.scale_log2 <= limit) && tile_top != -INFINITY)) {
+                float alpha = 1.0f;
+                if (tile_top * p.scale_log2 > limit) {
+                    alpha = ex2(fmaf(-tile_top, p.scale_log2, -shift));  // 0 for the first finite maximum
+                    if (top == -INFINITY) alpha = 0.0f;
+                    top = tile_top;
+                    shift = -top * p.scale_log2;
+                    limit = 8.0f - shift;
+                }
+                if (tile_top != tile_top) alpha = nan;  // a score is not a number: neither is the row
                 float a, b;
                 unpack2(sum2, &a, &b);
                 sum2 = pack2(a * alpha, b * alpha);
-            }
-            if (n > 0 && __any_sync(0xFFFFFFFFu, alpha < 1.0f)) {
+                if (n > 0) {
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + 32 * c, o);
-                    tmem_wait_ld();
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(t_o + 32 * c, o);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                    tmem_st32(t_o + 32 * c, o);
+                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        tmem_st32(t_o + 32 * c, o);
+                    }
                 }
             }
             const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), shift2 = pack2(shift, shift);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t pr[32];
+            for (int c = 0; c < 4; ++c) {
+                uint32_t pr[16];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    uint64_t x = ffma2(pack_u2(s[64 * c + 2 * e], s[64 * c + 2 * e + 1]), scale2, shift2);
+                for (int e = 0; e < 16; ++e) {
+                    uint32_t* pair = s + 32 * c + 2 * e;
+                    uint64_t x = ffma2(pack_u2(pair[0], pair[1]), scale2, shift2);
                     float a, b;
                     unpack2(x, &a, &b);
                     a = ex2(a), b = ex2(b);
-                    s[64 * c + 2 * e] = __float_as_uint(a), s[64 * c + 2 * e + 1] = __float_as_uint(b);
+                    pair[0] = __float_as_uint(a), pair[1] = __float_as_uint(b);
                     pr[e] = narrow2<kBf16>(a, b);
                 }
-                tmem_st32(t_s + 32 * c, pr);
+                tmem_st16(t_s + 16 * c, pr);
+                if (c & 1) {
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(smem_addr(&sm.p_full[stage][c >> 1]));
+                }
             }
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(smem_addr(&sm.p_full[stage]));
             // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over.
             uint64_t part[4] = {sum2, 0, 0, 0};
 #pragma unroll
@@ -544,11 +617,12 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         unpack2(sum2, &a, &b);
         const float sum = ok ? a + b : nan;
         if (kMode == kWhole) {
-            const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const bool none = top == -INFINITY && sum == sum;  // no key is visible
+            const float factor = none ? 0.0f : 1.0f / sum;
             const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
             if (real && p.lse != nullptr)
                 p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
-                    sum == 0.0f || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
+                    none || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
             uint4* dst = reinterpret_cast<uint4*>(p.out) + at * 16;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -573,7 +647,8 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             }
         } else {
             const long long slot = ((static_cast<long long>(item.index) * p.Hk + kv_head) * 2 + stage) * p.slot_rows + row;
-            if (real) p.part_ml[slot] = make_float2(sum == 0.0f ? -INFINITY : -shift, sum);
+            const bool none = top == -INFINITY && sum == sum;
+            if (real) p.part_ml[slot] = make_float2(none ? -INFINITY : -shift, none ? 0.0f : sum);
             float4* dst = reinterpret_cast<float4*>(p.part_o) + slot * 32;
             if (my_steps > 0 && ok) {
 #pragma unroll
