@@ -5,10 +5,13 @@
 // A row of the score tile is one query head of one token: the G query heads of a key head are packed behind each other
 // (row = token * G + head in group), 128 / G tokens to a tile of 128 rows, so that a key tile is read once for all of them.
 //
-// A CTA runs two softmax stages of 128 rows each (one row per thread).  Whole: the stages hold neighbouring tiles of rows
-// and both visit every key tile.  Split: an item is a range of key tiles; the CTA writes unnormalised partial results that
-// combine_kernel joins.  Wide split has the stages of the whole form; narrow split (at most one tile of rows per sequence)
-// gives both stages the same rows and every other key tile, since with one tile of rows the time goes into reading keys.
+// A CTA runs two softmax stages of 128 rows each (one row per thread).
+//   Whole: a CTA is two neighbouring tiles of rows with all their keys; both stages visit every key tile.
+//   Split, where that would leave SMs without work: the key tiles of all row tiles of all key heads are one list that is
+//   cut into equal shares, one to a CTA.  A share is one or a few segments (key tiles of one row tile), which the CTA
+//   works off one after another; it writes unnormalised partial results that combine_kernel joins.  Wide split has the
+//   stages of the whole form; narrow split (at most one tile of rows per sequence) gives both stages the same rows and every
+//   other key tile, since with one tile of rows the time goes into reading keys.
 //
 // Warp roles (384 threads): warps 0-3 / 4-7 softmax of stage 0 / 1, warp 8 TMA loads, warp 9 the products, warps 10 and
 // 11 clear the CTA's share of the rows behind the last sequence, where asked to.  Warp 8 also
@@ -42,7 +45,7 @@ constexpr int kSlots = 5;
 constexpr int kHalfBytes = kTile * 128;       // 128 rows of 64 values
 constexpr int kTileBytes = 2 * kHalfBytes;    // 128 rows of 128 values, as two halves of the channels
 constexpr uint32_t kColS = 0, kColO = 256, kTmemCols = 512;
-constexpr int kMaxTiles = 512;                // row tiles that a split launch can plan (shared memory)
+constexpr int kMaxTiles = 160;                // row tiles of a key head that a split launch can plan (shared memory)
 
 enum Mode { kWhole = 0, kSplitWide = 1, kSplitNarrow = 2 };
 
@@ -51,29 +54,28 @@ struct PackedParams {
     const int* cu_k;       // [B+1]
     void* out;             // [Tq,Hq,128]
     float* lse;            // [Hq,Tq] or null
-    float* part_o;         // split: [items * Hk * 2][slot_rows][128], unnormalised
-    float2* part_ml;       // split: [items * Hk * 2][slot_rows], (maximum in units of log2, sum)
+    float* part_o;         // split: [segments * 2][slot_rows][128], unnormalised
+    float2* part_ml;       // split: [segments * 2][slot_rows], (maximum in units of log2, sum)
     uint32_t* status;      // [1]: sticky word, or null
     volatile uint32_t* host_status;
     int B, Hq, Hk, G;
     int tokens;            // tokens of a tile of 128 rows: 128 / G
     int Tq, Tk;
-    int target, min_chunk; // split: wanted items per key head, least key tiles of an item
-    int max_tiles;         // split: row tiles that the workspace has room for
+    int ctas;              // split: shares
+    int max_tiles;         // split: row tiles of a key head that the workspace has room for
     int slot_rows;
     int zero_tail;         // rows behind the last sequence are set to zero
     float scale_log2;
 };
 
-// What a CTA works on: rows of one sequence and a range of its key tiles.
+// What a CTA works on: rows of one sequence, a key head and a range of the sequence's key tiles.
 struct Item {
-    int valid;             // 0: no such item
-    int index;
+    int valid;             // 0: nothing
+    int segment;           // split: where its partial results go
+    int kv_head;
     int q0, lq, k0, lk;    // the sequence
     int token0;            // first token of the tile within the sequence
     int t0, t1;            // key tiles
-    int first, count;      // split: the items of this row tile
-    int q_end;             // end of the last sequence
 };
 
 __device__ __forceinline__ void bounds(const int* cu, int b, int total, int* start, int* length) {
@@ -116,7 +118,7 @@ __device__ void find_tile(const PackedParams& p, int per_tile, int which, int la
         int all;
         const int at = before + warp_sum_before(n, lane, &all);
         if (which >= at && which < at + n) {
-            item->valid = 1, item->q0 = q0, item->lq = lq;
+            item->q0 = q0, item->lq = lq;
             bounds(p.cu_k, b, p.Tk, &item->k0, &item->lk);
             item->token0 = (n - 1 - (which - at)) * per_tile;
             item->t0 = 0;
@@ -125,82 +127,77 @@ __device__ void find_tile(const PackedParams& p, int per_tile, int which, int la
         found = which < before + all;
         before += all;
     }
-    if (lane == 0) {
-        item->index = which;
-        if (!found) item->valid = 0;
-        item->q_end = max(0, min(p.cu_q[p.B], p.Tq));
-    }
+    if (lane == 0) item->valid = found;
     __syncwarp();
 }
 
-// The plan of a split launch, made alike by every warp that asks: the key tiles of all row tiles are cut into pieces of
-// `chunk` (the same for all, so that long sequences get more CTAs than short ones and none waits for the longest), item
-// after item along the row tiles.  `which` counts items (by_item) or row tiles.
-struct PlanTile {
-    int seq, token0, key_tiles;
+// The row tiles of a key head (all key heads have the same) with the number of key tiles before each, made alike by every
+// warp that asks.  start[tiles] is the number of all.
+struct PlanTiles {
+    int count;
+    int seq[kMaxTiles], token0[kMaxTiles], start[kMaxTiles + 1];
 };
 template <bool kCausal>
-__device__ void find_split(const PackedParams& p, int per_tile, int which, bool by_item, int lane, PlanTile* list, Item* item) {
-    int tiles = 0;
-    long long total = 0;
+__device__ void plan_tiles(const PackedParams& p, int per_tile, int lane, PlanTiles* plan) {
+    int tiles = 0, total = 0;
     for (int base = 0; base < p.B; base += 32) {
         const int b = base + lane;
-        int q0 = 0, lq = 0, k0 = 0, lk = 0;
+        int q0, lq = 0, k0, lk = 0;
         if (b < p.B) {
             bounds(p.cu_q, b, p.Tq, &q0, &lq);
             bounds(p.cu_k, b, p.Tk, &k0, &lk);
         }
         // (More tiles than there is room for come of bounds that are out of order only.)
-        const int n = min((lq + per_tile - 1) / per_tile, kMaxTiles);
-        int all;
-        long long keys = 0;
+        int all, all_keys, n = min((lq + per_tile - 1) / per_tile, kMaxTiles);
         const int at = tiles + warp_sum_before(n, lane, &all);
-        for (int i = 0; i < n && at + i < p.max_tiles; ++i) {
-            list[at + i] = PlanTile{b, i * per_tile, visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile)};
-            keys += list[at + i].key_tiles;
+        n = max(0, min(n, p.max_tiles - at));
+        int keys = 0;
+        for (int i = 0; i < n; ++i) keys += visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile);
+        int start = total + warp_sum_before(keys, lane, &all_keys);
+        for (int i = 0; i < n; ++i) {
+            plan->seq[at + i] = b, plan->token0[at + i] = i * per_tile, plan->start[at + i] = start;
+            start += visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile);
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) keys += __shfl_xor_sync(0xFFFFFFFFu, keys, o);
-        total += keys;
         tiles = min(tiles + all, p.max_tiles);
+        total += all_keys;
     }
+    if (lane == 0) plan->count = tiles, plan->start[tiles] = total;
     __syncwarp();
-    const int chunk = max(p.min_chunk, static_cast<int>((total + p.target - 1) / p.target));
-    int before = 0;
-    bool found = false;
-    for (int base = 0; base < tiles && !found; base += 32) {
-        const int t = base + lane;
-        const int n = t < tiles ? (list[t].key_tiles + chunk - 1) / chunk : 0;
-        int all;
-        const int at = before + warp_sum_before(n, lane, &all);
-        if (by_item ? which >= at && which < at + n : t == which && t < tiles) {
-            const PlanTile tile = list[t];
-            item->valid = 1;
-            bounds(p.cu_q, tile.seq, p.Tq, &item->q0, &item->lq);
-            bounds(p.cu_k, tile.seq, p.Tk, &item->k0, &item->lk);
-            item->token0 = tile.token0;
-            item->first = at, item->count = n;
-            item->t0 = (which - at) * chunk;
-            item->t1 = min(item->t0 + chunk, tile.key_tiles);
-        }
-        before += all;
-        found = by_item ? which < before : which < base + 32 && which < tiles;
+}
+// The list of all key tiles (key head by key head) is cut into `shares` pieces, share c from (c * total) / shares.
+struct Shares {
+    long long total;
+    int shares;
+    __device__ Shares(const PlanTiles& plan, const PackedParams& p) {
+        total = static_cast<long long>(plan.start[plan.count]) * p.Hk;
+        shares = static_cast<int>(max(1LL, min(static_cast<long long>(p.ctas), total / 2)));  // of two tiles at least
     }
-    if (lane == 0) {
-        item->index = which;
-        if (!found) item->valid = 0;
-        item->q_end = max(0, min(p.cu_q[p.B], p.Tq));
+    __device__ long long first(int c) const { return c >= shares ? total : c * total / shares; }
+    __device__ int owner(long long at) const { return static_cast<int>(((at + 1) * shares + total - 1) / total) - 1; }
+};
+// The segment of share c that begins at `at` of the list.  Segments are counted by the shares and the row tiles before
+// them: each begins a share or a row tile.
+__device__ void find_segment(const PackedParams& p, const PlanTiles& plan, const Shares& shares, int c, long long at, int lane, Item* item) {
+    const int per_head = plan.start[plan.count], kv_head = static_cast<int>(at / per_head), r = static_cast<int>(at - static_cast<long long>(kv_head) * per_head);
+    for (int t = lane; t < plan.count; t += 32) {
+        if (r < plan.start[t] || r >= plan.start[t + 1]) continue;
+        item->valid = 1, item->kv_head = kv_head, item->segment = c + kv_head * plan.count + t;
+        bounds(p.cu_q, plan.seq[t], p.Tq, &item->q0, &item->lq);
+        bounds(p.cu_k, plan.seq[t], p.Tk, &item->k0, &item->lk);
+        item->token0 = plan.token0[t];
+        item->t0 = r - plan.start[t];
+        item->t1 = item->t0 + static_cast<int>(min(static_cast<long long>(plan.start[t + 1] - r), shares.first(c + 1) - at));
     }
     __syncwarp();
 }
 
-// Rows behind the last sequence: every CTA of a key head takes its share.
-__device__ __forceinline__ void clear_tail(const PackedParams& p, int q_end, int group0, int thread, int threads) {
-    for (long long t = q_end + static_cast<long long>(blockIdx.x); t < p.Tq; t += gridDim.x) {
-        uint4* dst = reinterpret_cast<uint4*>(p.out) + (t * p.Hq + group0) * 16;
-        for (int i = thread; i < p.G * 16; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
-        if (p.lse != nullptr)
-            for (int g = thread; g < p.G; g += threads) p.lse[static_cast<long long>(group0 + g) * p.Tq + t] = -INFINITY;
+// Rows behind the last sequence, every `stride`th from the `first`th: zero, -inf.
+__device__ __forceinline__ void clear_tail(const PackedParams& p, int first, int stride, int thread, int threads) {
+    const int q_end = max(0, min(p.cu_q[p.B], p.Tq));
+    for (long long t = q_end + static_cast<long long>(first); t < p.Tq; t += stride) {
+        uint4* dst = reinterpret_cast<uint4*>(p.out) + t * p.Hq * 16;
+        for (int i = thread; i < p.Hq * 16; i += threads) dst[i] = make_uint4(0, 0, 0, 0);
+        for (int h = thread; p.lse != nullptr && h < p.Hq; h += threads) p.lse[static_cast<long long>(h) * p.Tq + t] = -INFINITY;
     }
 }
 
@@ -285,6 +282,21 @@ __device__ __forceinline__ float max128_nan(const uint32_t (&s)[128]) {
     return fmax3_nan(fmax3_nan(m[0], m[1], m[2]), m[3], m[3]);
 }
 
+// Four lanes that hold four 16-byte pieces each of rows of their own exchange them: lane r of the four gets piece r of
+// every row, so that a store covers 64 bytes of eight rows and not 16 bytes of thirty-two (the output of 128 rows then
+// takes a quarter of the time: the store unit works through the rows of an instruction one by one).
+__device__ __forceinline__ void exchange4(uint4 (&u)[4], int lane) {
+    const auto swap = [](uint4& keep_low, uint4& keep_high, bool high, int mask) {
+        uint4 give = high ? keep_low : keep_high;
+        give.x = __shfl_xor_sync(0xFFFFFFFFu, give.x, mask), give.y = __shfl_xor_sync(0xFFFFFFFFu, give.y, mask);
+        give.z = __shfl_xor_sync(0xFFFFFFFFu, give.z, mask), give.w = __shfl_xor_sync(0xFFFFFFFFu, give.w, mask);
+        if (high) keep_low = give;
+        else keep_high = give;
+    };
+    swap(u[0], u[1], lane & 1, 1), swap(u[2], u[3], lane & 1, 1);
+    swap(u[0], u[2], lane & 2, 2), swap(u[1], u[3], lane & 2, 2);
+}
+
 struct Smem {
     alignas(1024) uint8_t q[2][kTileBytes];
     alignas(1024) uint8_t ring[kSlots][kTileBytes];
@@ -295,58 +307,63 @@ struct Smem {
     uint64_t o_full[2];
     uint64_t v_clean;                      // the rows behind the sequence's end are cleared in its last value tile
     uint64_t drain;
-    uint32_t tmem_base;
+    uint32_t tmem_base, gave_up;
     volatile uint32_t abort_flag;
+    Item item;
+    PlanTiles plan;
 };
 
 // The order in which a CTA visits key tiles.  Whole, wide: both stages every tile.  Narrow: stage s the tiles s, s + 2, ...
-// A tile is slot indices 2 i (K) and 2 i + 1 (V) of the ring, i counting the CTA's tiles.
+// A tile is slot indices 2 i (K) and 2 i + 1 (V) of the ring, i counting the segment's tiles.
 template <int kMode>
 __device__ __forceinline__ int tile_of(int stage, int n) {
     return kMode == kSplitNarrow ? 2 * n + stage : n;
+}
+
+// Steps of a stage.
+template <bool kCausal, int kMode>
+__device__ __forceinline__ int steps_of(const PackedParams& p, const Item& it, int stage) {
+    if (kMode == kSplitNarrow) return (it.t1 - it.t0 - stage + 1) / 2;
+    const int token = it.token0 + stage * p.tokens;
+    return token >= it.lq ? 0 : max(0, min(it.t1, visible_tiles<kCausal>(it.lq, it.lk, token, p.tokens)) - it.t0);
+}
+// Rows of the last value tile that belong to the sequence, where that is the sequence's last tile and not full; else 0.
+__device__ __forceinline__ int rows_to_keep(const Item& it) {
+    return it.t1 == (it.lk + kTile - 1) / kTile ? it.lk % kTile : 0;
 }
 
 template <bool kBf16, bool kCausal, int kMode>
 __global__ void __launch_bounds__(kThreads, 1)
 packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
               const __grid_constant__ CUtensorMap tmap_v, const __grid_constant__ PackedParams p) {
-    extern __shared__ uint8_t smem_raw[];
-    Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    __shared__ Item item;
-    __shared__ uint32_t gave_up;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];  // the kernel's only shared memory, so at the start of it
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+    constexpr bool kSplit = kMode != kWhole, kNarrow = kMode == kSplitNarrow;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kv_head = blockIdx.y;
-    const int per_cta = (kMode == kSplitNarrow ? 1 : 2) * p.tokens;  // tokens of a row tile
+    const int per_cta = (kNarrow ? 1 : 2) * p.tokens;  // tokens of a row tile
+    const float nan = __int_as_float(0x7FC00000);
+    const Item& item = sm.item;
 
     if (warp == 0) {
-        if (kMode == kWhole) find_tile<kCausal>(p, per_cta, blockIdx.x, lane, &item);
-        else find_split<kCausal>(p, per_cta, blockIdx.x, true, lane, reinterpret_cast<PlanTile*>(sm.q), &item);
-        // A barrier wait expired since the host last looked: start nothing, leave NaN.
-        if (lane == 0) gave_up = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
-    }
-    __syncthreads();
-    const int group0 = kv_head * p.G;  // first query head
-    const float nan = __int_as_float(0x7FC00000);
-
-    if (!item.valid) {  // an item beyond the last
-        if (kMode == kWhole && p.zero_tail) clear_tail(p, item.q_end, group0, threadIdx.x, kThreads);
-        return;
-    }
-
-    const int n_tiles = item.t1 - item.t0;
-    // Steps of each stage.
-    int steps[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-        if (kMode == kSplitNarrow) {
-            steps[s] = (n_tiles - s + 1) / 2;
-        } else {
-            const int token = item.token0 + s * p.tokens;
-            steps[s] = token >= item.lq ? 0 : max(0, min(item.t1, visible_tiles<kCausal>(item.lq, item.lk, token, p.tokens)) - item.t0);
+        // A barrier wait expired since the host last looked: start nothing, leave NaN.  (Nor could anything be computed
+        // were the tiles not on the 1024-byte grid of their swizzle.)
+        if (lane == 0) {
+            sm.gave_up = (p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u) | (smem_addr(smem_raw) & 1023u);
+            sm.abort_flag = 0;
         }
+        if (kSplit) plan_tiles<kCausal>(p, per_cta, lane, &sm.plan);
     }
-    const bool run = n_tiles > 0 && gave_up == 0;
+    if (warp == 9) {
+        tmem_alloc(smem_addr(&sm.tmem_base), kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    const bool live = sm.gave_up == 0;
+
     const auto wait = [&](uint64_t* bar, uint32_t parity) {
         return wait_bounded(&sm.abort_flag, bar, parity, kWaitCycles, [&] {
             sm.abort_flag = 1;
@@ -357,43 +374,46 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             }
         });
     };
-
-    uint32_t tmem = 0;
-    if (run) {
-        if (threadIdx.x == 0) {
-            for (int i = 0; i < 2; ++i) {
-                mbar_init(smem_addr(&sm.q_full[i]), 1);
-                mbar_init(smem_addr(&sm.s_full[i]), 1);
-                mbar_init(smem_addr(&sm.p_full[i][0]), 128);
-                mbar_init(smem_addr(&sm.p_full[i][1]), 128);
-                mbar_init(smem_addr(&sm.o_full[i]), 1);
+    // Where this CTA is in the list of key tiles (split), or whether its only item is still to come.
+    long long at = 0, end = 1, first_at = 0;
+    if (kSplit) {
+        const Shares shares(sm.plan, p);
+        at = first_at = shares.first(blockIdx.x), end = shares.first(blockIdx.x + 1);
+    }
+    // The next segment, for the whole CTA: false behind the last.  All products and copies of the one before are done.
+    const auto next_segment = [&]() {
+        if (at >= end) return false;
+        __syncwarp();
+        asm volatile("bar.sync 0;" ::: "memory");
+        if (warp == 0) {
+            if (kSplit) {
+                find_segment(p, sm.plan, Shares(sm.plan, p), blockIdx.x, at, lane, &sm.item);
+            } else {
+                find_tile<kCausal>(p, per_cta, blockIdx.x, lane, &sm.item);
+                if (lane == 0) sm.item.kv_head = blockIdx.y;
             }
-            for (int i = 0; i < kSlots; ++i) {
-                mbar_init(smem_addr(&sm.full[i]), 1);
-                mbar_init(smem_addr(&sm.empty[i]), 1);
+        }
+        if (threadIdx.x == 32) {
+            for (uint64_t* bar = sm.q_full; bar <= &sm.drain; ++bar) {
+                if (kSplit && at != first_at) mbar_inval(smem_addr(bar));
+                const bool by_stage = bar >= sm.p_full[0] && bar < sm.o_full;
+                mbar_init(smem_addr(bar), by_stage ? 128 : 1);
             }
-            mbar_init(smem_addr(&sm.v_clean), 1);
-            mbar_init(smem_addr(&sm.drain), 1);
-            sm.abort_flag = 0;
             mbar_init_fence();
         }
-        if (warp == 9) {
-            tmem_alloc(smem_addr(&sm.tmem_base), kTmemCols);
-            tmem_relinquish();
-        }
-        fence_proxy_async_smem();  // the plan was written where Q lands
-        tc_fence_before();
-        __syncthreads();
-        tc_fence_after();
-        tmem = sm.tmem_base;
-    }
-    // Keys of the last tile of this sequence; only an item that holds that tile has a value tile to clean.
-    const int last_tile = (item.lk + kTile - 1) / kTile - 1;
-    const int tail_rows = item.lk - last_tile * kTile;
-    const bool cleans = run && item.t1 - 1 == last_tile && tail_rows < kTile;
+        fence_proxy_async_smem();
+        __syncwarp();
+        asm volatile("bar.sync 0;" ::: "memory");
+        at += kSplit ? item.t1 - item.t0 : 1;
+        return item.valid != 0;
+    };
 
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        while (next_segment()) {
+        const int n_tiles = item.t1 - item.t0, kv_head = item.kv_head, group0 = kv_head * p.G, tail_rows = rows_to_keep(item);
+        const int steps[2] = {steps_of<kCausal, kMode>(p, item, 0), steps_of<kCausal, kMode>(p, item, 1)};
+        const bool cleans = tail_rows > 0, run = live && sm.abort_flag == 0 && n_tiles > 0;
         if (warp == 8 && run) {
             // ---------------- TMA loads ----------------
             const int q_tiles = kMode == kSplitNarrow ? 1 : 2;
@@ -514,21 +534,25 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 const long long t0 = clock64();
                 while (!mbar_try_wait(smem_addr(&sm.drain), 0) && clock64() - t0 < kWaitCycles) {}
             }
-        } else if (warp >= 10 && kMode == kWhole && p.zero_tail) {
-            clear_tail(p, item.q_end, group0, threadIdx.x - 320, 64);
         }
+        }
+        if (warp >= 10 && !kSplit && p.zero_tail)
+            clear_tail(p, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y, threadIdx.x - 320, 64);
     } else {
         // ---------------- softmax: one row per thread ----------------
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int stage = warp >> 2;
         const int row = (warp & 3) * 32 + lane;
+        while (next_segment()) {
+        const int group0 = item.kv_head * p.G;
         const int token = item.token0 + (kMode == kSplitNarrow ? 0 : stage * p.tokens) + row / p.G;  // within the sequence
         const int head = group0 + row % p.G;
         const bool real = row < p.tokens * p.G && token < item.lq;
         const int keys = kCausal ? max(0, min(item.lk, item.lk - item.lq + token + 1)) : item.lk;
         const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const uint32_t t_s = lane_base + kColS + 128 * stage, t_o = lane_base + kColO + 128 * stage;
-        const int my_steps = run ? steps[stage] : 0;
+        const bool go = live && sm.abort_flag == 0;
+        const int my_steps = go ? steps_of<kCausal, kMode>(p, item, stage) : 0;
 
         float top = -INFINITY;     // the maximum that the accumulator is scaled by
         float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
@@ -612,7 +636,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         }
         if (ok && my_steps > 0) ok = __all_sync(0xFFFFFFFFu, wait(&sm.o_full[stage], 0));
         tc_fence_after();
-        ok = ok && gave_up == 0;
+        ok = ok && go;
         float a, b;
         unpack2(sum2, &a, &b);
         const float sum = ok ? a + b : nan;
@@ -623,7 +647,12 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             if (real && p.lse != nullptr)
                 p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
                     none || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
-            uint4* dst = reinterpret_cast<uint4*>(p.out) + at * 16;
+            // After the exchange a lane stores its piece of the four rows of its group.
+            uint4* to[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                to[i] = reinterpret_cast<uint4*>(p.out) + __shfl_sync(0xFFFFFFFFu, real ? at : -1LL, (lane & ~3) + i) * 16 + (lane & 3);
+            const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 uint32_t o[32];
@@ -634,45 +663,54 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0;
                 }
-                if (real) {
+                uint4 u[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t w[4];
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
-                        dst[4 * c + e] = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
+                    u[e] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
+                exchange4(u, lane);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (reals >> i & 1) to[i][4 * c] = u[i];
             }
         } else {
-            const long long slot = ((static_cast<long long>(item.index) * p.Hk + kv_head) * 2 + stage) * p.slot_rows + row;
+            const long long slot = (static_cast<long long>(item.segment) * 2 + stage) * p.slot_rows + row;
             const bool none = top == -INFINITY && sum == sum;
             if (real) p.part_ml[slot] = make_float2(none ? -INFINITY : -shift, none ? 0.0f : sum);
-            float4* dst = reinterpret_cast<float4*>(p.part_o) + slot * 32;
+            const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
+            const bool any_real = __any_sync(0xFFFFFFFFu, real);
+            uint4* const to = reinterpret_cast<uint4*>(p.part_o) + (slot - (lane & 3)) * 32 + (lane & 3);
             if (my_steps > 0 && ok) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t o[32];
                     tmem_ld32(t_o + 32 * c, o);
                     tmem_wait_ld();
-                    if (real) {
+                    if (!any_real) continue;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e)
-                            dst[8 * c + e] = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                                         __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                    for (int h = 0; h < 2; ++h) {
+                        uint4 u[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[e] = make_uint4(o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
+                        exchange4(u, lane);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (reals >> i & 1) to[32 * i + 8 * c + 4 * h] = u[i];
                     }
                 }
             }
         }
-    }
-    if (run) {
-        tc_fence_before();
-        __syncthreads();
-        if (warp == 9) {
-            tc_fence_after();
-            tmem_dealloc(tmem, kTmemCols);
         }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
     }
 }
 
@@ -681,24 +719,33 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 // A partial that saw no key has l = 0 and its O was not written.
 template <bool kBf16, bool kCausal, bool kNarrow>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ PackedParams p) {
-    __shared__ Item item;
-    __shared__ PlanTile list[kMaxTiles];
+    __shared__ PlanTiles plan;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kv_head = blockIdx.y, group0 = kv_head * p.G;
     const int per_cta = (kNarrow ? 1 : 2) * p.tokens;
-    if (warp == 0) find_split<kCausal>(p, per_cta, blockIdx.x, false, lane, list, &item);
+    if (warp == 0) plan_tiles<kCausal>(p, per_cta, lane, &plan);
     __syncthreads();
-    if (p.zero_tail && blockIdx.z == 0) clear_tail(p, item.q_end, group0, threadIdx.x, 256);
-    if (!item.valid) return;
-    const int rows = min(per_cta, item.lq - item.token0) * p.G;
+    if (p.zero_tail && kv_head == 0 && blockIdx.z == 0) clear_tail(p, blockIdx.x, gridDim.x, threadIdx.x, 256);
+    const int tile = blockIdx.x;
+    if (tile >= plan.count) return;
+    int q0, lq;
+    bounds(p.cu_q, plan.seq[tile], p.Tq, &q0, &lq);
+    const Shares shares(plan, p);
+    // The shares that the tile's keys lie in, none where it has none.
+    const long long from = static_cast<long long>(kv_head) * plan.start[plan.count] + plan.start[tile];
+    const int key_tiles = plan.start[tile + 1] - plan.start[tile];
+    const int share0 = key_tiles > 0 ? shares.owner(from) : 0;
+    const int segments = key_tiles > 0 ? shares.owner(from + key_tiles - 1) - share0 + 1 : 0;
+    const int segment0 = share0 + kv_head * plan.count + tile;
+    const int token0 = plan.token0[tile], rows = min(per_cta, lq - token0) * p.G;
     for (int r = blockIdx.z * 8 + warp; r < rows; r += 8 * gridDim.z) {
         // Row r of the row tile is row r of its only 128-row tile, or of the second one.
         const int stage = kNarrow ? 0 : r / (p.tokens * p.G);
         const int slot_row = r - stage * p.tokens * p.G;
-        const int parts = item.count * (kNarrow ? 2 : 1);
+        const int parts = segments * (kNarrow ? 2 : 1);
         const auto slot = [&](int i) {
-            const int index = item.first + (kNarrow ? i >> 1 : i), s = kNarrow ? i & 1 : stage;
-            return ((static_cast<long long>(index) * p.Hk + kv_head) * 2 + s) * p.slot_rows + slot_row;
+            const int segment = segment0 + (kNarrow ? i >> 1 : i), s = kNarrow ? i & 1 : stage;
+            return (static_cast<long long>(segment) * 2 + s) * p.slot_rows + slot_row;
         };
         float top = -INFINITY;
         for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
@@ -717,7 +764,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
             acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
         }
         const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const long long t = item.q0 + item.token0 + r / p.G;
+        const long long t = q0 + token0 + r / p.G;
         const int head = group0 + r % p.G;
         reinterpret_cast<uint2*>(p.out)[(t * p.Hq + head) * 32 + lane] =
             make_uint2(narrow2<kBf16>(acc.x * factor, acc.y * factor), narrow2<kBf16>(acc.z * factor, acc.w * factor));
@@ -749,35 +796,34 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int6
 
 // How a launch is laid out; from sizes alone (the lengths of the sequences are on the device).
 struct Layout {
-    int mode, tokens, slot_rows, target, min_chunk;
-    int64_t tiles;  // at most so many row tiles per key head
-    int64_t items;  // split: at most so many items per key head
+    int mode, tokens, slot_rows;
+    int64_t tiles;     // at most so many row tiles per key head
+    int64_t segments;  // split: at most so many segments
 };
 
+constexpr int64_t kSms = 148;
+
 Layout lay_out(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
-    constexpr int64_t kSms = 148;
     Layout l{};
     const int64_t G = Hq / Hk;
     l.tokens = static_cast<int>(kTile / G);
     // n sequences of at least one token make at most Tq tiles, and at most one tile each that is not full.
     const auto tiles = [&](int64_t per_tile) { const int64_t t = Tq / per_tile + B; return t < Tq ? t : Tq; };
-    l.mode = kWhole, l.tiles = tiles(2 * l.tokens), l.items = l.tiles;
+    l.mode = kWhole, l.tiles = tiles(2 * l.tokens);
     // Split where whole row tiles leave SMs without work and there are keys enough to share.
     const int64_t key_tiles = ceil_div(Tk, kTile);
     if (l.tiles * Hk < kSms && l.tiles <= kMaxTiles && key_tiles >= 4 * B) {
         l.mode = kSplitWide;
         if (Tq * G <= kTile * B && tiles(l.tokens) <= kMaxTiles) l.mode = kSplitNarrow, l.tiles = tiles(l.tokens);
-        l.target = static_cast<int>(ceil_div(2 * kSms, Hk));
-        l.min_chunk = 2;
-        l.items = l.target + l.tiles;
+        l.segments = kSms + l.tiles * Hk;
         const int64_t rows = Tq * G;
         l.slot_rows = static_cast<int>(rows < kTile ? rows : kTile);
     }
     return l;
 }
 
-int64_t workspace_bytes(const Layout& l, int64_t Hk) {
-    return l.mode == kWhole ? 0 : l.items * Hk * 2 * l.slot_rows * (kDim + 2) * static_cast<int64_t>(sizeof(float));
+int64_t workspace_bytes(const Layout& l) {
+    return l.mode == kWhole ? 0 : l.segments * 2 * l.slot_rows * (kDim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 bool bad_sizes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
@@ -792,7 +838,7 @@ using namespace ovc;
 
 extern "C" int64_t ovc_attention_packed_workspace(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
     if (bad_sizes(B, Tq, Tk, Hq, Hk)) return 0;
-    return workspace_bytes(lay_out(B, Tq, Tk, Hq, Hk), Hk);
+    return workspace_bytes(lay_out(B, Tq, Tk, Hq, Hk));
 }
 
 extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -807,7 +853,7 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     for (const int64_t* s : {q_strides, k_strides, v_strides})
         if (s[0] <= 0 || s[1] <= 0 || s[0] % 8 || s[1] % 8 || s[0] >= (1LL << 38) || s[1] >= (1LL << 38)) return OVC_ERR_ARGUMENT;
     const Layout l = lay_out(B, Tq, Tk, Hq, Hk);
-    if (workspace_bytes(l, Hk) > 0 && (!workspace || !aligned16(workspace))) return OVC_ERR_ARGUMENT;
+    if (workspace_bytes(l) > 0 && (!workspace || !aligned16(workspace))) return OVC_ERR_ARGUMENT;
 
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
@@ -828,17 +874,18 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     PackedParams p{};
     p.cu_q = cu_seqlens_q, p.cu_k = cu_seqlens_k, p.out = out, p.lse = lse;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (l.mode == kWhole ? 0 : l.items * Hk * 2 * l.slot_rows * kDim));
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (l.mode == kWhole ? 0 : l.segments * 2 * l.slot_rows * kDim));
     p.status = status, p.host_status = host_status;
     p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.Hk = static_cast<int>(Hk), p.G = static_cast<int>(G);
     p.tokens = l.tokens, p.Tq = static_cast<int>(Tq), p.Tk = static_cast<int>(Tk);
-    p.target = l.target, p.min_chunk = l.min_chunk, p.max_tiles = static_cast<int>(l.tiles < kMaxTiles ? l.tiles : kMaxTiles), p.slot_rows = l.slot_rows;
+    p.ctas = static_cast<int>(kSms), p.max_tiles = static_cast<int>(l.tiles < kMaxTiles ? l.tiles : kMaxTiles), p.slot_rows = l.slot_rows;
     p.zero_tail = (flags & OVC_ATTN_ZERO_TAIL) != 0;
     p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
 
-    constexpr int smem = sizeof(Smem) + 1024;
+    constexpr int smem = sizeof(Smem);
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto s = static_cast<cudaStream_t>(stream);
-    const dim3 grid(static_cast<unsigned>(l.items), static_cast<unsigned>(Hk));
+    const dim3 grid(static_cast<unsigned>(l.mode == kWhole ? l.tiles : kSms), static_cast<unsigned>(l.mode == kWhole ? Hk : 1));
     const auto launch = [&](auto kernel) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) { set_last_cuda_error(e); return static_cast<int>(OVC_ERR_CUDA); }
@@ -851,8 +898,8 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
         const int r = l.mode == kSplitNarrow ? launch(packed_kernel<kB, kC, kSplitNarrow>) : launch(packed_kernel<kB, kC, kSplitWide>);
         if (r != OVC_OK) return r;
         const int rows = (l.mode == kSplitNarrow ? 1 : 2) * l.tokens * static_cast<int>(G);
-        const int64_t rows_all = Tq * G < rows ? Tq * G : rows;
-        const dim3 cgrid(static_cast<unsigned>(l.tiles), static_cast<unsigned>(Hk), static_cast<unsigned>(ceil_div(rows_all, 8)));
+        const int64_t mean = ceil_div(Tq * G, B);  // rows of a sequence; a row tile has them, or is full
+        const dim3 cgrid(static_cast<unsigned>(l.tiles), static_cast<unsigned>(Hk), static_cast<unsigned>(ceil_div(mean < rows ? mean : rows, 16)));
         if (l.mode == kSplitNarrow) combine_kernel<kB, kC, true><<<cgrid, 256, 0, s>>>(p);
         else combine_kernel<kB, kC, false><<<cgrid, 256, 0, s>>>(p);
         return check_launch();
