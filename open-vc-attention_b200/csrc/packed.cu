@@ -49,11 +49,19 @@ constexpr int kMaxTiles = 160;                // row tiles of a key head that a 
 
 enum Mode { kWhole = 0, kSplitWide = 1, kSplitNarrow = 2 };
 
+// The row tiles of a key head (all key heads have the same), made alike by every warp that asks, and what each costs: a unit
+// for each of its key tiles and segment_cost more.  start[t] is the sum before tile t, start[count] of all.
+struct PlanTiles {
+    int count;
+    int seq[kMaxTiles], token0[kMaxTiles], start[kMaxTiles + 1];
+};
+
 struct PackedParams {
     const int* cu_q;       // [B+1]
     const int* cu_k;       // [B+1]
     void* out;             // [Tq,Hq,128]
     float* lse;            // [Hq,Tq] or null
+    PlanTiles* plan;       // split: for combine_kernel
     float* part_o;         // split: [segments * 2][slot_rows][128], unnormalised
     float2* part_ml;       // split: [segments * 2][slot_rows], (maximum in units of log2, sum)
     uint32_t* status;      // [1]: sticky word, or null
@@ -62,6 +70,7 @@ struct PackedParams {
     int tokens;            // tokens of a tile of 128 rows: 128 / G
     int Tq, Tk;
     int ctas;              // split: shares
+    int segment_cost;      // split: what it costs to begin and end a segment, in key tiles
     int max_tiles;         // split: row tiles of a key head that the workspace has room for
     int slot_rows;
     int zero_tail;         // rows behind the last sequence are set to zero
@@ -76,6 +85,7 @@ struct Item {
     int q0, lq, k0, lk;    // the sequence
     int token0;            // first token of the tile within the sequence
     int t0, t1;            // key tiles
+    int units;             // split: how far it is along the list
 };
 
 __device__ __forceinline__ void bounds(const int* cu, int b, int total, int* start, int* length) {
@@ -131,12 +141,7 @@ __device__ void find_tile(const PackedParams& p, int per_tile, int which, int la
     __syncwarp();
 }
 
-// The row tiles of a key head (all key heads have the same) with the number of key tiles before each, made alike by every
-// warp that asks.  start[tiles] is the number of all.
-struct PlanTiles {
-    int count;
-    int seq[kMaxTiles], token0[kMaxTiles], start[kMaxTiles + 1];
-};
+__device__ __forceinline__ int tile_cost(const PackedParams& p, int key_tiles) { return key_tiles > 0 ? key_tiles + p.segment_cost : 0; }
 template <bool kCausal>
 __device__ void plan_tiles(const PackedParams& p, int per_tile, int lane, PlanTiles* plan) {
     int tiles = 0, total = 0;
@@ -148,46 +153,59 @@ __device__ void plan_tiles(const PackedParams& p, int per_tile, int lane, PlanTi
             bounds(p.cu_k, b, p.Tk, &k0, &lk);
         }
         // (More tiles than there is room for come of bounds that are out of order only.)
-        int all, all_keys, n = min((lq + per_tile - 1) / per_tile, kMaxTiles);
+        int all, all_costs, n = min((lq + per_tile - 1) / per_tile, kMaxTiles);
         const int at = tiles + warp_sum_before(n, lane, &all);
         n = max(0, min(n, p.max_tiles - at));
-        int keys = 0;
-        for (int i = 0; i < n; ++i) keys += visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile);
-        int start = total + warp_sum_before(keys, lane, &all_keys);
+        int cost = 0;
+        for (int i = 0; i < n; ++i) cost += tile_cost(p, visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile));
+        int start = total + warp_sum_before(cost, lane, &all_costs);
         for (int i = 0; i < n; ++i) {
             plan->seq[at + i] = b, plan->token0[at + i] = i * per_tile, plan->start[at + i] = start;
-            start += visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile);
+            start += tile_cost(p, visible_tiles<kCausal>(lq, lk, i * per_tile, per_tile));
         }
         tiles = min(tiles + all, p.max_tiles);
-        total += all_keys;
+        total += all_costs;
     }
     if (lane == 0) plan->count = tiles, plan->start[tiles] = total;
     __syncwarp();
 }
-// The list of all key tiles (key head by key head) is cut into `shares` pieces, share c from (c * total) / shares.
+// The list of all units (key head by key head) is cut into `shares` pieces, share c from (c * total) / shares.
 struct Shares {
     long long total;
     int shares;
     __device__ Shares(const PlanTiles& plan, const PackedParams& p) {
         total = static_cast<long long>(plan.start[plan.count]) * p.Hk;
-        shares = static_cast<int>(max(1LL, min(static_cast<long long>(p.ctas), total / 2)));  // of two tiles at least
+        shares = static_cast<int>(max(1LL, min(static_cast<long long>(p.ctas), total / (2 + p.segment_cost))));  // of two tiles at least
     }
     __device__ long long first(int c) const { return c >= shares ? total : c * total / shares; }
     __device__ int owner(long long at) const { return static_cast<int>(((at + 1) * shares + total - 1) / total) - 1; }
 };
-// The segment of share c that begins at `at` of the list.  Segments are counted by the shares and the row tiles before
-// them: each begins a share or a row tile.
+// The first segment of share c from `at` of the list on.  Of a row tile's units the first segment_cost are no key tiles: a
+// piece of those alone is no segment.  Segments are counted by the shares and the row tiles before them (each begins
+// either).
 __device__ void find_segment(const PackedParams& p, const PlanTiles& plan, const Shares& shares, int c, long long at, int lane, Item* item) {
-    const int per_head = plan.start[plan.count], kv_head = static_cast<int>(at / per_head), r = static_cast<int>(at - static_cast<long long>(kv_head) * per_head);
-    for (int t = lane; t < plan.count; t += 32) {
-        if (r < plan.start[t] || r >= plan.start[t + 1]) continue;
-        item->valid = 1, item->kv_head = kv_head, item->segment = c + kv_head * plan.count + t;
-        bounds(p.cu_q, plan.seq[t], p.Tq, &item->q0, &item->lq);
-        bounds(p.cu_k, plan.seq[t], p.Tk, &item->k0, &item->lk);
-        item->token0 = plan.token0[t];
-        item->t0 = r - plan.start[t];
-        item->t1 = item->t0 + static_cast<int>(min(static_cast<long long>(plan.start[t + 1] - r), shares.first(c + 1) - at));
+    const int per_head = plan.start[plan.count];
+    const long long end = shares.first(c + 1);
+    long long pos = at;
+    bool found = false;
+    while (pos < end && !found) {
+        const int kv_head = static_cast<int>(pos / per_head), r = static_cast<int>(pos - static_cast<long long>(kv_head) * per_head);
+        int units = 0;
+        for (int t = lane; t < plan.count; t += 32) {
+            if (r < plan.start[t] || r >= plan.start[t + 1]) continue;
+            units = static_cast<int>(min(static_cast<long long>(plan.start[t + 1] - r), end - pos));
+            const int from = r - plan.start[t] - p.segment_cost, t0 = max(0, from), t1 = max(0, from + units);
+            if (t1 <= t0) continue;
+            found = true;
+            item->kv_head = kv_head, item->segment = c + kv_head * plan.count + t;
+            bounds(p.cu_q, plan.seq[t], p.Tq, &item->q0, &item->lq);
+            bounds(p.cu_k, plan.seq[t], p.Tk, &item->k0, &item->lk);
+            item->token0 = plan.token0[t], item->t0 = t0, item->t1 = t1;
+        }
+        found = __any_sync(0xFFFFFFFFu, found);
+        pos += static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(units)));
     }
+    if (lane == 0) item->valid = found, item->units = static_cast<int>(pos - at);
     __syncwarp();
 }
 
@@ -374,6 +392,10 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             }
         });
     };
+    if (kSplit && blockIdx.x == 0 && warp == 10) {
+        const int* from = reinterpret_cast<const int*>(&sm.plan);
+        for (int i = lane; i < static_cast<int>(sizeof(PlanTiles) / sizeof(int)); i += 32) reinterpret_cast<int*>(p.plan)[i] = from[i];
+    }
     // Where this CTA is in the list of key tiles (split), or whether its only item is still to come.
     long long at = 0, end = 1, first_at = 0;
     if (kSplit) {
@@ -404,7 +426,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         fence_proxy_async_smem();
         __syncwarp();
         asm volatile("bar.sync 0;" ::: "memory");
-        at += kSplit ? item.t1 - item.t0 : 1;
+        at += kSplit ? item.units : 1;
         return item.valid != 0;
     };
 
@@ -717,14 +739,12 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 // Joins the partial results of a split launch: a warp per row, four channels per lane.
 //   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i,  lse = ln 2 (M + log2 of that sum).
 // A partial that saw no key has l = 0 and its O was not written.
-template <bool kBf16, bool kCausal, bool kNarrow>
+template <bool kBf16, bool kNarrow>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ PackedParams p) {
-    __shared__ PlanTiles plan;
+    const PlanTiles& plan = *p.plan;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kv_head = blockIdx.y, group0 = kv_head * p.G;
     const int per_cta = (kNarrow ? 1 : 2) * p.tokens;
-    if (warp == 0) plan_tiles<kCausal>(p, per_cta, lane, &plan);
-    __syncthreads();
     if (p.zero_tail && kv_head == 0 && blockIdx.z == 0) clear_tail(p, blockIdx.x, gridDim.x, threadIdx.x, 256);
     const int tile = blockIdx.x;
     if (tile >= plan.count) return;
@@ -733,9 +753,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
     const Shares shares(plan, p);
     // The shares that the tile's keys lie in, none where it has none.
     const long long from = static_cast<long long>(kv_head) * plan.start[plan.count] + plan.start[tile];
-    const int key_tiles = plan.start[tile + 1] - plan.start[tile];
-    const int share0 = key_tiles > 0 ? shares.owner(from) : 0;
-    const int segments = key_tiles > 0 ? shares.owner(from + key_tiles - 1) - share0 + 1 : 0;
+    const int cost = plan.start[tile + 1] - plan.start[tile];
+    const int share0 = cost > 0 ? shares.owner(from + p.segment_cost) : 0;
+    const int segments = cost > 0 ? shares.owner(from + cost - 1) - share0 + 1 : 0;
     const int segment0 = share0 + kv_head * plan.count + tile;
     const int token0 = plan.token0[tile], rows = min(per_cta, lq - token0) * p.G;
     for (int r = blockIdx.z * 8 + warp; r < rows; r += 8 * gridDim.z) {
@@ -822,8 +842,9 @@ Layout lay_out(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
     return l;
 }
 
+constexpr int64_t kPlanBytes = (sizeof(PlanTiles) + 255) / 256 * 256;
 int64_t workspace_bytes(const Layout& l) {
-    return l.mode == kWhole ? 0 : l.segments * 2 * l.slot_rows * (kDim + 2) * static_cast<int64_t>(sizeof(float));
+    return l.mode == kWhole ? 0 : kPlanBytes + l.segments * 2 * l.slot_rows * (kDim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 bool bad_sizes(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
@@ -873,11 +894,16 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
 
     PackedParams p{};
     p.cu_q = cu_seqlens_q, p.cu_k = cu_seqlens_k, p.out = out, p.lse = lse;
-    p.part_o = static_cast<float*>(workspace);
+    p.plan = static_cast<PlanTiles*>(workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (l.mode == kWhole ? 0 : kPlanBytes));
     p.part_ml = reinterpret_cast<float2*>(p.part_o + (l.mode == kWhole ? 0 : l.segments * 2 * l.slot_rows * kDim));
     p.status = status, p.host_status = host_status;
     p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.Hk = static_cast<int>(Hk), p.G = static_cast<int>(G);
     p.tokens = l.tokens, p.Tq = static_cast<int>(Tq), p.Tk = static_cast<int>(Tk);
+    // Narrow: a segment's beginning and end take as long as about four key tiles (with 0, 2, 4, 6 of them sixteen requests
+    // of 129 to 32768 keys took 109, 100, 93, 93 us).  Wide: a key tile takes three times as long, and is cheaper where only
+    // one stage has rows; shares by key tiles alone were the best (0: 218 us, 2: 223, 4: 233 for chunks behind prefixes).
+    p.segment_cost = l.mode == kSplitNarrow ? 4 : 0;
     p.ctas = static_cast<int>(kSms), p.max_tiles = static_cast<int>(l.tiles < kMaxTiles ? l.tiles : kMaxTiles), p.slot_rows = l.slot_rows;
     p.zero_tail = (flags & OVC_ATTN_ZERO_TAIL) != 0;
     p.scale_log2 = static_cast<float>(static_cast<double>(softmax_scale) * 1.4426950408889634);
@@ -900,8 +926,8 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
         const int rows = (l.mode == kSplitNarrow ? 1 : 2) * l.tokens * static_cast<int>(G);
         const int64_t mean = ceil_div(Tq * G, B);  // rows of a sequence; a row tile has them, or is full
         const dim3 cgrid(static_cast<unsigned>(l.tiles), static_cast<unsigned>(Hk), static_cast<unsigned>(ceil_div(mean < rows ? mean : rows, 16)));
-        if (l.mode == kSplitNarrow) combine_kernel<kB, kC, true><<<cgrid, 256, 0, s>>>(p);
-        else combine_kernel<kB, kC, false><<<cgrid, 256, 0, s>>>(p);
+        if (l.mode == kSplitNarrow) combine_kernel<kB, true><<<cgrid, 256, 0, s>>>(p);
+        else combine_kernel<kB, false><<<cgrid, 256, 0, s>>>(p);
         return check_launch();
     };
     if (bf16) return causal ? by_mask(std::true_type{}, std::true_type{}) : by_mask(std::true_type{}, std::false_type{});
