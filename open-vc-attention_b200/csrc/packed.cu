@@ -433,130 +433,130 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         while (next_segment()) {
-        const int n_tiles = item.t1 - item.t0, kv_head = item.kv_head, group0 = kv_head * p.G, tail_rows = rows_to_keep(item);
-        const int steps[2] = {steps_of<kCausal, kMode>(p, item, 0), steps_of<kCausal, kMode>(p, item, 1)};
-        const bool cleans = tail_rows > 0, run = live && sm.abort_flag == 0 && n_tiles > 0;
-        if (warp == 8 && run) {
-            // ---------------- TMA loads ----------------
-            const int q_tiles = kMode == kSplitNarrow ? 1 : 2;
-            int issued = 0;
-            if (lane == 0) {
-                tma_prefetch_desc(&tmap_k);
-                tma_prefetch_desc(&tmap_v);
-                const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
-                const uint64_t kv_policy = kMode == kSplitNarrow ? stream : keep;
-                const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128;  // of one half
-                for (int s = 0; s < q_tiles; ++s) {
-                    mbar_expect_tx(smem_addr(&sm.q_full[s]), 2 * q_bytes);
-                    const int token = item.q0 + item.token0 + s * p.tokens;
-                    for (int h = 0; h < 2; ++h)
-                        tma_load_4d(smem_addr(sm.q[s]) + h * kHalfBytes, &tmap_q, smem_addr(&sm.q_full[s]), 0, group0, token, h, stream);
+            const int n_tiles = item.t1 - item.t0, kv_head = item.kv_head, group0 = kv_head * p.G, tail_rows = rows_to_keep(item);
+            const int steps[2] = {steps_of<kCausal, kMode>(p, item, 0), steps_of<kCausal, kMode>(p, item, 1)};
+            const bool cleans = tail_rows > 0, run = live && sm.abort_flag == 0 && n_tiles > 0;
+            if (warp == 8 && run) {
+                // ---------------- TMA loads ----------------
+                const int q_tiles = kMode == kSplitNarrow ? 1 : 2;
+                int issued = 0;
+                if (lane == 0) {
+                    tma_prefetch_desc(&tmap_k);
+                    tma_prefetch_desc(&tmap_v);
+                    const uint64_t keep = policy_evict_last(), stream = policy_evict_first();
+                    const uint64_t kv_policy = kMode == kSplitNarrow ? stream : keep;
+                    const uint32_t q_bytes = static_cast<uint32_t>(p.tokens * p.G) * 128;  // of one half
+                    for (int s = 0; s < q_tiles; ++s) {
+                        mbar_expect_tx(smem_addr(&sm.q_full[s]), 2 * q_bytes);
+                        const int token = item.q0 + item.token0 + s * p.tokens;
+                        for (int h = 0; h < 2; ++h)
+                            tma_load_4d(smem_addr(sm.q[s]) + h * kHalfBytes, &tmap_q, smem_addr(&sm.q_full[s]), 0, group0, token, h, stream);
+                    }
+                    for (int i = 0; i < 2 * n_tiles; ++i) {
+                        const int slot = i % kSlots;
+                        if (i >= kSlots && !wait(&sm.empty[slot], (i / kSlots - 1) & 1)) break;
+                        mbar_expect_tx(smem_addr(&sm.full[slot]), kTileBytes);
+                        const int key = item.k0 + (item.t0 + (i >> 1)) * kTile;
+                        tma_load_4d(smem_addr(sm.ring[slot]), (i & 1) ? &tmap_v : &tmap_k, smem_addr(&sm.full[slot]), 0, kv_head, key, 0, kv_policy);
+                        issued = i + 1;
+                    }
                 }
-                for (int i = 0; i < 2 * n_tiles; ++i) {
-                    const int slot = i % kSlots;
-                    if (i >= kSlots && !wait(&sm.empty[slot], (i / kSlots - 1) & 1)) break;
-                    mbar_expect_tx(smem_addr(&sm.full[slot]), kTileBytes);
-                    const int key = item.k0 + (item.t0 + (i >> 1)) * kTile;
-                    tma_load_4d(smem_addr(sm.ring[slot]), (i & 1) ? &tmap_v : &tmap_k, smem_addr(&sm.full[slot]), 0, kv_head, key, 0, kv_policy);
-                    issued = i + 1;
+                issued = __shfl_sync(0xFFFFFFFFu, issued, 0);
+                // The last value tile: its rows behind the end of the sequence.  (The warp that issued the load may wait for
+                // it: its slot's earlier phases are over, so the parity is unambiguous.)
+                const int index = 2 * n_tiles - 1;
+                if (cleans && issued == 2 * n_tiles && __all_sync(0xFFFFFFFFu, wait(&sm.full[index % kSlots], (index / kSlots) & 1))) {
+                    for (int h = 0; h < 2; ++h) {
+                        uint4* rows = reinterpret_cast<uint4*>(sm.ring[index % kSlots] + h * kHalfBytes);
+                        for (int i = tail_rows * 8 + lane; i < kTile * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_addr(&sm.v_clean));
                 }
-            }
-            issued = __shfl_sync(0xFFFFFFFFu, issued, 0);
-            // The last value tile: its rows behind the end of the sequence.  (The warp that issued the load may wait for
-            // it: its slot's earlier phases are over, so the parity is unambiguous.)
-            const int index = 2 * n_tiles - 1;
-            if (cleans && issued == 2 * n_tiles && __all_sync(0xFFFFFFFFu, wait(&sm.full[index % kSlots], (index / kSlots) & 1))) {
-                for (int h = 0; h < 2; ++h) {
-                    uint4* rows = reinterpret_cast<uint4*>(sm.ring[index % kSlots] + h * kHalfBytes);
-                    for (int i = tail_rows * 8 + lane; i < kTile * 8; i += 32) rows[i] = make_uint4(0, 0, 0, 0);
+                // Every copy has landed before the CTA's shared memory goes away (it has, unless a wait expired).
+                if (lane == 0) {
+                    const long long t0 = clock64();
+                    for (int i = max(0, issued - kSlots); i < issued; ++i)
+                        while (!mbar_try_wait(smem_addr(&sm.full[i % kSlots]), (i / kSlots) & 1) && clock64() - t0 < kWaitCycles) {}
+                    for (int s = 0; s < q_tiles; ++s)
+                        while (!mbar_try_wait(smem_addr(&sm.q_full[s]), 0) && clock64() - t0 < kWaitCycles) {}
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_addr(&sm.v_clean));
-            }
-            // Every copy has landed before the CTA's shared memory goes away (it has, unless a wait expired).
-            if (lane == 0) {
-                const long long t0 = clock64();
-                for (int i = max(0, issued - kSlots); i < issued; ++i)
-                    while (!mbar_try_wait(smem_addr(&sm.full[i % kSlots]), (i / kSlots) & 1) && clock64() - t0 < kWaitCycles) {}
-                for (int s = 0; s < q_tiles; ++s)
-                    while (!mbar_try_wait(smem_addr(&sm.q_full[s]), 0) && clock64() - t0 < kWaitCycles) {}
-            }
-        } else if (warp == 9 && run) {
-            // ---------------- products ----------------
-            // One warp issues for both stages, in a fixed order, which keeps them half a step apart (with a warp for each
-            // stage they drifted into step: 1.25 times the time).  The issuing lane is held until all but the last
-            // products have run, so what lies between two issues is kept short: slots and descriptors are carried along,
-            // the copies are waited for by the first stage that needs them (in the narrow form, where keys are what is
-            // waited for, K of the next step only once V's slot is on its way back).
-            constexpr uint32_t id_qk = idesc<kBf16>(false), id_pv = idesc<kBf16>(true);
-            const auto uniform = [](int x) { return static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(x))); };
-            const int steps0 = uniform(steps[0]), steps1 = uniform(steps[1]), dirty = uniform(cleans ? n_tiles : 0) - 1;
-            const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
-            const auto all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)) != 0; };
-            struct Slot {
-                int i = 0;
-                uint32_t phase = 0;
-                __device__ __forceinline__ void advance() { if (++i == kSlots) i = 0, phase ^= 1; }
-            };
-            const uint32_t ring_lo = smem_desc_lo(smem_addr(sm.ring[0])), q_lo = smem_desc_lo(smem_addr(sm.q[0]));
-            const uint32_t ring_lo_mn = smem_desc_lo_bmn(smem_addr(sm.ring[0]), kHalfBytes);
-            const auto scores = [&](int s, const Slot& k, bool last_reader) {
-                product_qk(tm + kColS + 128 * s, q_lo + (kMode == kSplitNarrow ? 0 : s * (kTileBytes >> 4)), ring_lo + k.i * (kTileBytes >> 4), id_qk);
-                mma_commit_elect(smem_addr(&sm.s_full[s]));
-                if (last_reader) mma_commit_elect(smem_addr(&sm.empty[k.i]));
-            };
-            // Slots of K of a stage's next step and V of its present one.
-            Slot k, v;
-            v.advance();
-            bool ok = true;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (ok && (s ? steps1 : steps0) > 0) {
-                    ok = all(&sm.q_full[kMode == kSplitNarrow ? 0 : s], 0) && all(&sm.full[k.i], k.phase);
-                    if (ok) scores(s, k, kMode == kSplitNarrow || s == 1 || steps1 == 0);
-                }
-                if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance();
-            }
-            const int most = max(steps0, steps1);
-            for (int n = 0; ok && n < most; ++n) {
+            } else if (warp == 9 && run) {
+                // ---------------- products ----------------
+                // One warp issues for both stages, in a fixed order, which keeps them half a step apart (with a warp for each
+                // stage they drifted into step: 1.25 times the time).  The issuing lane is held until all but the last
+                // products have run, so what lies between two issues is kept short: slots and descriptors are carried along,
+                // the copies are waited for by the first stage that needs them (in the narrow form, where keys are what is
+                // waited for, K of the next step only once V's slot is on its way back).
+                constexpr uint32_t id_qk = idesc<kBf16>(false), id_pv = idesc<kBf16>(true);
+                const auto uniform = [](int x) { return static_cast<int>(__reduce_max_sync(0xFFFFFFFFu, static_cast<unsigned>(x))); };
+                const int steps0 = uniform(steps[0]), steps1 = uniform(steps[1]), dirty = uniform(cleans ? n_tiles : 0) - 1;
+                const uint32_t tm = static_cast<uint32_t>(uniform(static_cast<int>(tmem)));
+                const auto all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait(bar, parity)) != 0; };
+                struct Slot {
+                    int i = 0;
+                    uint32_t phase = 0;
+                    __device__ __forceinline__ void advance() { if (++i == kSlots) i = 0, phase ^= 1; }
+                };
+                const uint32_t ring_lo = smem_desc_lo(smem_addr(sm.ring[0])), q_lo = smem_desc_lo(smem_addr(sm.q[0]));
+                const uint32_t ring_lo_mn = smem_desc_lo_bmn(smem_addr(sm.ring[0]), kHalfBytes);
+                const auto scores = [&](int s, const Slot& k, bool last_reader) {
+                    product_qk(tm + kColS + 128 * s, q_lo + (kMode == kSplitNarrow ? 0 : s * (kTileBytes >> 4)), ring_lo + k.i * (kTileBytes >> 4), id_qk);
+                    mma_commit_elect(smem_addr(&sm.s_full[s]));
+                    if (last_reader) mma_commit_elect(smem_addr(&sm.empty[k.i]));
+                };
+                // Slots of K of a stage's next step and V of its present one.
+                Slot k, v;
+                v.advance();
+                bool ok = true;
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const int mine = s ? steps1 : steps0;
-                    if (n < mine) {
-                        const uint32_t t_o = tm + kColO + 128 * s, t_p = tm + kColS + 128 * s, v_lo = ring_lo_mn + v.i * (kTileBytes >> 4);
-                        const bool first = kMode == kSplitNarrow || s == 0 || n >= steps0, last = kMode == kSplitNarrow || s == 1 || n >= steps1;
-                        const bool more = n + 1 < mine;
-                        if (first) {
-                            ok = all(&sm.full[v.i], v.phase) && (tile_of<kMode>(s, n) != dirty || all(&sm.v_clean, 0));
-                            if (kMode != kSplitNarrow && more) ok = ok && all(&sm.full[k.i], k.phase);
-                        } else if (more && n + 1 >= steps0) {
-                            ok = all(&sm.full[k.i], k.phase);
-                        }
-                        // The first half of the keys is multiplied while the stage still works on the second.
-                        ok = ok && all(&sm.p_full[s][0], n & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        product_pv(t_o, t_p, v_lo, id_pv, n > 0);
-                        ok = all(&sm.p_full[s][1], n & 1);
-                        if (!ok) break;
-                        tc_fence_after();
-                        product_pv(t_o, t_p + 32, v_lo + 512, id_pv, 1);
-                        if (last) mma_commit_elect(smem_addr(&sm.empty[v.i]));
-                        if (kMode == kSplitNarrow && more) ok = all(&sm.full[k.i], k.phase);
-                        if (!ok) break;
-                        if (more) scores(s, k, kMode == kSplitNarrow || s == 1 || n + 1 >= steps1);
-                        else mma_commit_elect(smem_addr(&sm.o_full[s]));
+                    if (ok && (s ? steps1 : steps0) > 0) {
+                        ok = all(&sm.q_full[kMode == kSplitNarrow ? 0 : s], 0) && all(&sm.full[k.i], k.phase);
+                        if (ok) scores(s, k, kMode == kSplitNarrow || s == 1 || steps1 == 0);
                     }
-                    if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance(), v.advance(), v.advance();
+                    if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance();
+                }
+                const int most = max(steps0, steps1);
+                for (int n = 0; ok && n < most; ++n) {
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const int mine = s ? steps1 : steps0;
+                        if (n < mine) {
+                            const uint32_t t_o = tm + kColO + 128 * s, t_p = tm + kColS + 128 * s, v_lo = ring_lo_mn + v.i * (kTileBytes >> 4);
+                            const bool first = kMode == kSplitNarrow || s == 0 || n >= steps0, last = kMode == kSplitNarrow || s == 1 || n >= steps1;
+                            const bool more = n + 1 < mine;
+                            if (first) {
+                                ok = all(&sm.full[v.i], v.phase) && (tile_of<kMode>(s, n) != dirty || all(&sm.v_clean, 0));
+                                if (kMode != kSplitNarrow && more) ok = ok && all(&sm.full[k.i], k.phase);
+                            } else if (more && n + 1 >= steps0) {
+                                ok = all(&sm.full[k.i], k.phase);
+                            }
+                            // The first half of the keys is multiplied while the stage still works on the second.
+                            ok = ok && all(&sm.p_full[s][0], n & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            product_pv(t_o, t_p, v_lo, id_pv, n > 0);
+                            ok = all(&sm.p_full[s][1], n & 1);
+                            if (!ok) break;
+                            tc_fence_after();
+                            product_pv(t_o, t_p + 32, v_lo + 512, id_pv, 1);
+                            if (last) mma_commit_elect(smem_addr(&sm.empty[v.i]));
+                            if (kMode == kSplitNarrow && more) ok = all(&sm.full[k.i], k.phase);
+                            if (!ok) break;
+                            if (more) scores(s, k, kMode == kSplitNarrow || s == 1 || n + 1 >= steps1);
+                            else mma_commit_elect(smem_addr(&sm.o_full[s]));
+                        }
+                        if (kMode == kSplitNarrow || s == 1) k.advance(), k.advance(), v.advance(), v.advance();
+                    }
+                }
+                if (!ok) {  // products in flight end before tensor memory is released
+                    mma_commit_elect(smem_addr(&sm.drain));
+                    const long long t0 = clock64();
+                    while (!mbar_try_wait(smem_addr(&sm.drain), 0) && clock64() - t0 < kWaitCycles) {}
                 }
             }
-            if (!ok) {  // products in flight end before tensor memory is released
-                mma_commit_elect(smem_addr(&sm.drain));
-                const long long t0 = clock64();
-                while (!mbar_try_wait(smem_addr(&sm.drain), 0) && clock64() - t0 < kWaitCycles) {}
-            }
-        }
         }
         if (warp >= 10 && !kSplit && p.zero_tail)
             clear_tail(p, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y, threadIdx.x - 320, 64);
@@ -566,166 +566,166 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const int stage = warp >> 2;
         const int row = (warp & 3) * 32 + lane;
         while (next_segment()) {
-        const int group0 = item.kv_head * p.G;
-        const int token = item.token0 + (kMode == kSplitNarrow ? 0 : stage * p.tokens) + row / p.G;  // within the sequence
-        const int head = group0 + row % p.G;
-        const bool real = row < p.tokens * p.G && token < item.lq;
-        const int keys = kCausal ? max(0, min(item.lk, item.lk - item.lq + token + 1)) : item.lk;
-        const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
-        const uint32_t t_s = lane_base + kColS + 128 * stage, t_o = lane_base + kColO + 128 * stage;
-        const bool go = live && sm.abort_flag == 0;
-        const int my_steps = go ? steps_of<kCausal, kMode>(p, item, stage) : 0;
+            const int group0 = item.kv_head * p.G;
+            const int token = item.token0 + (kMode == kSplitNarrow ? 0 : stage * p.tokens) + row / p.G;  // within the sequence
+            const int head = group0 + row % p.G;
+            const bool real = row < p.tokens * p.G && token < item.lq;
+            const int keys = kCausal ? max(0, min(item.lk, item.lk - item.lq + token + 1)) : item.lk;
+            const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+            const uint32_t t_s = lane_base + kColS + 128 * stage, t_o = lane_base + kColO + 128 * stage;
+            const bool go = live && sm.abort_flag == 0;
+            const int my_steps = go ? steps_of<kCausal, kMode>(p, item, stage) : 0;
 
-        float top = -INFINITY;     // the maximum that the accumulator is scaled by
-        float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
-        float limit = -INFINITY;   // a scaled score above it moves the maximum
-        // Steps whose tile every row of the warp sees in full.
-        const int whole_tiles = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(keys))) / kTile - item.t0;
-        const int whole_steps = kMode == kSplitNarrow ? (whole_tiles - stage + 1) / 2 : whole_tiles;
-        uint64_t sum2 = 0;         // the running sum, even and odd columns
-        bool ok = true;
-        for (int n = 0; n < my_steps; ++n) {
-            ok = __all_sync(0xFFFFFFFFu, wait(&sm.s_full[stage], n & 1));
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t s[128];
-            tmem_ld32(t_s, s);
-            tmem_ld32(t_s + 32, s + 32);
-            tmem_ld32(t_s + 64, s + 64);
-            tmem_ld32(t_s + 96, s + 96);
-            tmem_wait_ld();
-            if (n >= whole_steps) {
-                const int columns = keys - (item.t0 + tile_of<kMode>(stage, n)) * kTile;
+            float top = -INFINITY;     // the maximum that the accumulator is scaled by
+            float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
+            float limit = -INFINITY;   // a scaled score above it moves the maximum
+            // Steps whose tile every row of the warp sees in full.
+            const int whole_tiles = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(keys))) / kTile - item.t0;
+            const int whole_steps = kMode == kSplitNarrow ? (whole_tiles - stage + 1) / 2 : whole_tiles;
+            uint64_t sum2 = 0;         // the running sum, even and odd columns
+            bool ok = true;
+            for (int n = 0; n < my_steps; ++n) {
+                ok = __all_sync(0xFFFFFFFFu, wait(&sm.s_full[stage], n & 1));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[128];
+                tmem_ld32(t_s, s);
+                tmem_ld32(t_s + 32, s + 32);
+                tmem_ld32(t_s + 64, s + 64);
+                tmem_ld32(t_s + 96, s + 96);
+                tmem_wait_ld();
+                if (n >= whole_steps) {
+                    const int columns = keys - (item.t0 + tile_of<kMode>(stage, n)) * kTile;
 #pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    if (c >= columns) s[c] = 0xFF800000u;  // -inf, whatever the key holds
-            }
-            // The maximum moves only when it grows by more than 2^8: until then probabilities above 1 are as exact as those
-            // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.  The
-            // comparison is false where both are -inf (no key yet) and true where a score is not a number.
-            const float tile_top = max128_nan(s);
-            if (__any_sync(0xFFFFFFFFu, !(tile_top * p.scale_log2 <= limit) && tile_top != -INFINITY)) {
-                float alpha = 1.0f;
-                if (tile_top * p.scale_log2 > limit) {
-                    alpha = ex2(fmaf(-tile_top, p.scale_log2, -shift));  // 0 for the first finite maximum
-                    if (top == -INFINITY) alpha = 0.0f;
-                    top = tile_top;
-                    shift = -top * p.scale_log2;
-                    limit = 8.0f - shift;
+                    for (int c = 0; c < 128; ++c)
+                        if (c >= columns) s[c] = 0xFF800000u;  // -inf, whatever the key holds
                 }
-                if (tile_top != tile_top) alpha = nan;  // a score is not a number: neither is the row
-                float a, b;
-                unpack2(sum2, &a, &b);
-                sum2 = pack2(a * alpha, b * alpha);
-                if (n > 0) {
+                // The maximum moves only when it grows by more than 2^8: until then probabilities above 1 are as exact as those
+                // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.  The
+                // comparison is false where both are -inf (no key yet) and true where a score is not a number.
+                const float tile_top = max128_nan(s);
+                if (__any_sync(0xFFFFFFFFu, !(tile_top * p.scale_log2 <= limit) && tile_top != -INFINITY)) {
+                    float alpha = 1.0f;
+                    if (tile_top * p.scale_log2 > limit) {
+                        alpha = ex2(fmaf(-tile_top, p.scale_log2, -shift));  // 0 for the first finite maximum
+                        if (top == -INFINITY) alpha = 0.0f;
+                        top = tile_top;
+                        shift = -top * p.scale_log2;
+                        limit = 8.0f - shift;
+                    }
+                    if (tile_top != tile_top) alpha = nan;  // a score is not a number: neither is the row
+                    float a, b;
+                    unpack2(sum2, &a, &b);
+                    sum2 = pack2(a * alpha, b * alpha);
+                    if (n > 0) {
 #pragma unroll 1
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t o[32];
+                            tmem_ld32(t_o + 32 * c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                            tmem_st32(t_o + 32 * c, o);
+                        }
+                    }
+                }
+                const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), shift2 = pack2(shift, shift);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t pr[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint32_t* pair = s + 32 * c + 2 * e;
+                        uint64_t x = ffma2(pack_u2(pair[0], pair[1]), scale2, shift2);
+                        float a, b;
+                        unpack2(x, &a, &b);
+                        a = ex2(a), b = ex2(b);
+                        pair[0] = __float_as_uint(a), pair[1] = __float_as_uint(b);
+                        pr[e] = narrow2<kBf16>(a, b);
+                    }
+                    tmem_st16(t_s + 16 * c, pr);
+                    if (c & 1) {
+                        tmem_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(smem_addr(&sm.p_full[stage][c >> 1]));
+                    }
+                }
+                // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over.
+                uint64_t part[4] = {sum2, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 64; ++e) part[e & 3] = fadd2(part[e & 3], pack_u2(s[2 * e], s[2 * e + 1]));
+                sum2 = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
+            }
+            if (ok && my_steps > 0) ok = __all_sync(0xFFFFFFFFu, wait(&sm.o_full[stage], 0));
+            tc_fence_after();
+            ok = ok && go;
+            float a, b;
+            unpack2(sum2, &a, &b);
+            const float sum = ok ? a + b : nan;
+            if (kMode == kWhole) {
+                const bool none = top == -INFINITY && sum == sum;  // no key is visible
+                const float factor = none ? 0.0f : 1.0f / sum;
+                const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
+                if (real && p.lse != nullptr)
+                    p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
+                        none || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
+                // After the exchange a lane stores its piece of the four rows of its group.
+                uint4* to[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    to[i] = reinterpret_cast<uint4*>(p.out) + __shfl_sync(0xFFFFFFFFu, real ? at : -1LL, (lane & ~3) + i) * 16 + (lane & 3);
+                const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t o[32];
+                    if (my_steps > 0 && ok) {  // warp-uniform
+                        tmem_ld32(t_o + 32 * c, o);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0;
+                    }
+                    uint4 u[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
+                        u[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    exchange4(u, lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (reals >> i & 1) to[i][4 * c] = u[i];
+                }
+            } else {
+                const long long slot = (static_cast<long long>(item.segment) * 2 + stage) * p.slot_rows + row;
+                const bool none = top == -INFINITY && sum == sum;
+                if (real) p.part_ml[slot] = make_float2(none ? -INFINITY : -shift, none ? 0.0f : sum);
+                const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
+                const bool any_real = __any_sync(0xFFFFFFFFu, real);
+                uint4* const to = reinterpret_cast<uint4*>(p.part_o) + (slot - (lane & 3)) * 32 + (lane & 3);
+                if (my_steps > 0 && ok) {
+#pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t o[32];
                         tmem_ld32(t_o + 32 * c, o);
                         tmem_wait_ld();
+                        if (!any_real) continue;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-                        tmem_st32(t_o + 32 * c, o);
+                        for (int h = 0; h < 2; ++h) {
+                            uint4 u[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) u[e] = make_uint4(o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
+                            exchange4(u, lane);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (reals >> i & 1) to[32 * i + 8 * c + 4 * h] = u[i];
+                        }
                     }
                 }
             }
-            const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), shift2 = pack2(shift, shift);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t pr[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    uint32_t* pair = s + 32 * c + 2 * e;
-                    uint64_t x = ffma2(pack_u2(pair[0], pair[1]), scale2, shift2);
-                    float a, b;
-                    unpack2(x, &a, &b);
-                    a = ex2(a), b = ex2(b);
-                    pair[0] = __float_as_uint(a), pair[1] = __float_as_uint(b);
-                    pr[e] = narrow2<kBf16>(a, b);
-                }
-                tmem_st16(t_s + 16 * c, pr);
-                if (c & 1) {
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(smem_addr(&sm.p_full[stage][c >> 1]));
-                }
-            }
-            // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over.
-            uint64_t part[4] = {sum2, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 64; ++e) part[e & 3] = fadd2(part[e & 3], pack_u2(s[2 * e], s[2 * e + 1]));
-            sum2 = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
-        }
-        if (ok && my_steps > 0) ok = __all_sync(0xFFFFFFFFu, wait(&sm.o_full[stage], 0));
-        tc_fence_after();
-        ok = ok && go;
-        float a, b;
-        unpack2(sum2, &a, &b);
-        const float sum = ok ? a + b : nan;
-        if (kMode == kWhole) {
-            const bool none = top == -INFINITY && sum == sum;  // no key is visible
-            const float factor = none ? 0.0f : 1.0f / sum;
-            const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
-            if (real && p.lse != nullptr)
-                p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
-                    none || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
-            // After the exchange a lane stores its piece of the four rows of its group.
-            uint4* to[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                to[i] = reinterpret_cast<uint4*>(p.out) + __shfl_sync(0xFFFFFFFFu, real ? at : -1LL, (lane & ~3) + i) * 16 + (lane & 3);
-            const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t o[32];
-                if (my_steps > 0 && ok) {  // warp-uniform
-                    tmem_ld32(t_o + 32 * c, o);
-                    tmem_wait_ld();
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0;
-                }
-                uint4 u[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
-                    u[e] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
-                exchange4(u, lane);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (reals >> i & 1) to[i][4 * c] = u[i];
-            }
-        } else {
-            const long long slot = (static_cast<long long>(item.segment) * 2 + stage) * p.slot_rows + row;
-            const bool none = top == -INFINITY && sum == sum;
-            if (real) p.part_ml[slot] = make_float2(none ? -INFINITY : -shift, none ? 0.0f : sum);
-            const uint32_t reals = __ballot_sync(0xFFFFFFFFu, real) >> (lane & ~3);
-            const bool any_real = __any_sync(0xFFFFFFFFu, real);
-            uint4* const to = reinterpret_cast<uint4*>(p.part_o) + (slot - (lane & 3)) * 32 + (lane & 3);
-            if (my_steps > 0 && ok) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(t_o + 32 * c, o);
-                    tmem_wait_ld();
-                    if (!any_real) continue;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint4 u[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] = make_uint4(o[16 * h + 4 * e], o[16 * h + 4 * e + 1], o[16 * h + 4 * e + 2], o[16 * h + 4 * e + 3]);
-                        exchange4(u, lane);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (reals >> i & 1) to[32 * i + 8 * c + 4 * h] = u[i];
-                    }
-                }
-            }
-        }
         }
     }
     tc_fence_before();
@@ -814,6 +814,20 @@ int make_map(CUtensorMap* map, const void* base, bool bf16, int64_t tokens, int6
     return OVC_OK;
 }
 
+// The current device; whether the library's code runs there (asked for once per device).
+int sm100_device(int* device) {
+    static std::atomic<unsigned long long> known;
+    cudaError_t err = cudaGetDevice(device);
+    if (err == cudaSuccess && *device < 64 && known.load(std::memory_order_acquire) >> *device & 1) return OVC_OK;
+    int major = 0, minor = 0;
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *device);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, *device);
+    if (err != cudaSuccess) { set_last_cuda_error(err); return OVC_ERR_CUDA; }
+    if (major != 10 || minor != 0) return OVC_ERR_UNSUPPORTED;
+    if (*device < 64) known.fetch_or(1ull << *device, std::memory_order_release);
+    return OVC_OK;
+}
+
 // How a launch is laid out; from sizes alone (the lengths of the sequences are on the device).
 struct Layout {
     int mode, tokens, slot_rows;
@@ -877,12 +891,8 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     if (workspace_bytes(l) > 0 && (!workspace || !aligned16(workspace))) return OVC_ERR_ARGUMENT;
 
     int device = 0;
-    cudaError_t err = cudaGetDevice(&device);
-    int major = 0, minor = 0;
-    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
-    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device);
-    if (err != cudaSuccess) { set_last_cuda_error(err); return OVC_ERR_CUDA; }
-    if (major != 10 || minor != 0) return OVC_ERR_UNSUPPORTED;
+    const int supported = sm100_device(&device);
+    if (supported != OVC_OK) return supported;
 
     const bool bf16 = dtype == OVC_BF16, causal = (flags & OVC_ATTN_CAUSAL) != 0;
     const int64_t G = Hq / Hk;
@@ -912,16 +922,21 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto s = static_cast<cudaStream_t>(stream);
     const dim3 grid(static_cast<unsigned>(l.mode == kWhole ? l.tiles : kSms), static_cast<unsigned>(l.mode == kWhole ? Hk : 1));
-    const auto launch = [&](auto kernel) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) { set_last_cuda_error(e); return static_cast<int>(OVC_ERR_CUDA); }
+    const auto launch = [&](auto kernel, auto* ready) {  // ready: the devices on which the kernel may take that much
+        if (device >= 64 || !(ready->load(std::memory_order_acquire) >> device & 1)) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (e != cudaSuccess) { set_last_cuda_error(e); return static_cast<int>(OVC_ERR_CUDA); }
+            if (device < 64) ready->fetch_or(1ull << device, std::memory_order_release);
+        }
         kernel<<<grid, kThreads, smem, s>>>(map_q, map_k, map_v, p);
         return check_launch();
     };
     const auto by_mask = [&](auto is_bf16, auto is_causal) {
         constexpr bool kB = decltype(is_bf16)::value, kC = decltype(is_causal)::value;
-        if (l.mode == kWhole) return launch(packed_kernel<kB, kC, kWhole>);
-        const int r = l.mode == kSplitNarrow ? launch(packed_kernel<kB, kC, kSplitNarrow>) : launch(packed_kernel<kB, kC, kSplitWide>);
+        static std::atomic<unsigned long long> ready[3];
+        if (l.mode == kWhole) return launch(packed_kernel<kB, kC, kWhole>, &ready[kWhole]);
+        const int r = l.mode == kSplitNarrow ? launch(packed_kernel<kB, kC, kSplitNarrow>, &ready[kSplitNarrow])
+                                             : launch(packed_kernel<kB, kC, kSplitWide>, &ready[kSplitWide]);
         if (r != OVC_OK) return r;
         const int rows = (l.mode == kSplitNarrow ? 1 : 2) * l.tokens * static_cast<int>(G);
         const int64_t mean = ceil_div(Tq * G, B);  // rows of a sequence; a row tile has them, or is full

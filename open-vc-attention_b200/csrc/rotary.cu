@@ -17,6 +17,7 @@
 
 #include <math.h>
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -545,7 +546,13 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     auto s = static_cast<cudaStream_t>(stream);
     const auto launch = [&](auto bf16, auto half, auto norm) {
         const auto kernel = rotary_quant_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>;
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        static std::atomic<unsigned long long> ready;  // devices on which the kernel may take that much
+        int device = 0;
+        cudaError_t err = cudaGetDevice(&device);
+        if (err == cudaSuccess && (device >= 64 || !(ready.load(std::memory_order_acquire) >> device & 1))) {
+            err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (err == cudaSuccess && device < 64) ready.fetch_or(1ull << device, std::memory_order_release);
+        }
         if (err != cudaSuccess) { set_last_cuda_error(err); return static_cast<int>(OVC_ERR_CUDA); }
         kernel<<<grid, kQuantThreads, smem, s>>>(a, static_cast<int>(blocks), per_cta);
         return check_launch();

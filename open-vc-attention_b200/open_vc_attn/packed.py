@@ -15,16 +15,22 @@ from . import _lib
 from .forward import _raise_if_flagged, _status
 
 
-def _strides(t):
-    """Elements from one token and one head of [T,H,128] to the next; None where the rows cannot be read in place."""
-    if t.stride(2) != 1 or t.data_ptr() % 16:
+def _in_place(t):
+    """(pointer, C array of the elements from one token and one head of [T,H,128] to the next); None where the rows cannot be
+    read in place."""
+    token, head, channel = t.stride()
+    pointer = t.data_ptr()
+    if channel != 1 or pointer % 16:
         return None
     # the stride of a single token or head is never used, and may be anything
-    token = t.stride(0) if t.shape[0] > 1 else 128 * t.shape[1]
-    head = t.stride(1) if t.shape[1] > 1 else 128
+    tokens, heads, _ = t.shape
+    if tokens == 1:
+        token = 128 * heads
+    if heads == 1:
+        head = 128
     if token <= 0 or head <= 0 or token % 8 or head % 8:
         return None
-    return token, head
+    return pointer, (ctypes.c_int64 * 2)(token, head)
 
 
 def _check_bounds(name, cu, device):
@@ -55,10 +61,12 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     Stream ordered, no synchronisation, capturable.  As for ``attention``, a launch whose bounded waits expire leaves NaN and is
     reported by a later call or by ``forward.check_status``.
     """
-    if any(t.ndim != 3 or t.shape[-1] != 128 for t in (q, k, v)):
+    if q.ndim != 3 or k.ndim != 3:
         raise ValueError("Expected packed [T,H,128] Q/K/V")
-    tq, hq, _ = q.shape
-    tk, hk, _ = k.shape
+    tq, hq, dim_q = q.shape
+    tk, hk, dim_k = k.shape
+    if dim_q != 128 or dim_k != 128:
+        raise ValueError("Expected packed [T,H,128] Q/K/V")
     if k.shape != v.shape:
         raise ValueError("K and V shapes must match")
     if hk < 1 or hq < hk or hq % hk or hq // hk > 128:
@@ -93,7 +101,7 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     with _lib.on_device(device):
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        lse = torch.empty((hq, tq), dtype=torch.float32, device=device) if return_lse else None
+        lse = q.new_empty((hq, tq), dtype=torch.float32) if return_lse else None
         if tq == 0:
             return (out, lse) if return_lse else out
         if tk == 0:
@@ -106,19 +114,19 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
             return (out, lse.fill_(-math.inf)) if return_lse else out
         arguments, keep = [], []
         for t in (q, k, v):
-            strides = _strides(t)
-            if strides is None:
+            read = _in_place(t)
+            if read is None:
                 t = t.clone(memory_format=torch.contiguous_format)
-                strides = (t.shape[1] * 128, 128)
-            keep.append(t)
-            arguments += [t.data_ptr(), (ctypes.c_int64 * 2)(*strides)]
+                keep.append(t)
+                read = _in_place(t)
+            arguments += read
         sizes = (cu_seqlens_q.shape[0] - 1, tq, tk, hq, hk)
         size = lib.ovc_attention_packed_workspace(*sizes)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         words, mirror = _status(device)
         _lib.check(
             lib.ovc_attention_packed(
-                *arguments, _lib.dtype_code(q.dtype), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *sizes, flags,
+                *arguments, _lib.OVC_BF16 if q.dtype == torch.bfloat16 else _lib.OVC_F16, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *sizes, flags,
                 softmax_scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
                 None if workspace is None else workspace.data_ptr(), words.data_ptr() + 4, mirror.data_ptr(),
                 _lib.raw_stream(device.index),
