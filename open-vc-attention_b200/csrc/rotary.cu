@@ -116,7 +116,6 @@ __device__ __forceinline__ void in_order(const Four& v, float (&f)[8]) {
         f[kHalf ? 4 + i : 2 * i + 1] = b[i];
     }
 }
-// (The library wants weights on a 16-byte boundary.)
 template <bool kHalf>
 __device__ __forceinline__ Four load_weights(const float* weight, int c16) {
     const float4 x = reinterpret_cast<const float4*>(weight)[kHalf ? c16 : 2 * c16];
@@ -221,7 +220,7 @@ struct RotaryArgs {
     float* amax_init;                    // rotary_quant_kernel: optional [H], set to 0
 };
 
-constexpr int kUnitRows = 32, kUnitWarps = 4, kGroupRows = 8;
+constexpr int kGroupRows = 8, kUnitGroups = 4, kUnitWarps = 4;
 
 // 16 bytes to shared memory behind the thread's back: what is in flight takes no registers.
 __device__ __forceinline__ void copy16(void* to, const void* from) {
@@ -232,44 +231,40 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// HBM bound: 4 bytes per element (2 read, 2 written).  A warp takes up to 32 heads of one token (those of q, then those of
-// k), asks for all of them at once, computes the token's angles meanwhile - four pairs to a lane, kept in registers - and
-// then works through the heads eight at a time, two side by side, as they arrive.
+// HBM bound: 4 bytes per element (2 read, 2 written).  The heads of a token's q and then of its k are groups of eight, a unit
+// is up to four groups of one token.  A warp asks for all heads of its unit at once, computes the token's angles meanwhile -
+// four pairs to a lane, kept in registers - and then works through the groups as they arrive, two heads side by side.
+// Measured with groups of one tensor each against heads of either in a row, which cost every head a choice of pointers and
+// weights: 122 and 143 us for [4, 8191, 24 + 24, 128] with norm (805 MB; a copy of that size takes 123 us).
 template <int DT, bool kHalf, bool kNorm>
-__global__ void __launch_bounds__(32 * kUnitWarps, 7) rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_rows, int units) {
+__global__ void __launch_bounds__(32 * kUnitWarps, 7)
+rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int unit_groups) {
     extern __shared__ __align__(16) uint8_t staged[];
     __shared__ Pairs pairs;
-    __shared__ __align__(16) float weights[2][kDim];
     const int lane = threadIdx.x & 31, c16 = lane & 15, side = lane >> 4;
     const long long unit = static_cast<long long>(blockIdx.x) * kUnitWarps + (threadIdx.x >> 5);
     const long long wanted = unit / units, token = min(wanted, a.tokens - 1);
+    const int groups0 = (a.src[0].heads + kGroupRows - 1) / kGroupRows, all = groups0 + (a.src[1].heads + kGroupRows - 1) / kGroupRows;
+    const int first = static_cast<int>(unit - wanted * units) * unit_groups;
+    const int count = wanted < a.tokens ? min(unit_groups, all - first) : 0;
     const long long b = token / a.S, s = token - b * a.S;
-    const int q_heads = a.src[0].heads;
-    const int first = static_cast<int>(unit - wanted * units) * unit_rows;
-    const int rows = wanted < a.tokens ? min(unit_rows, q_heads + a.src[1].heads - first) : 0;
-    uint8_t* const mine = staged + (threadIdx.x >> 5) * unit_rows * 256;
+    uint8_t* const mine = staged + (threadIdx.x >> 5) * unit_groups * kGroupRows * 256;
 
-    const uint16_t* const xq = a.src[0].x + b * a.src[0].batch + s * a.src[0].token + 8 * c16;
-    const uint16_t* const xk = a.src[1].x + b * a.src[1].batch + s * a.src[1].token + 8 * c16;
 #pragma unroll
-    for (int g = 0; g < kUnitRows; g += kGroupRows) {
+    for (int j = 0; j < kUnitGroups; ++j) {
+        if (j < count) {
+            const Source& t = a.src[first + j >= groups0];
+            const int head = (first + j >= groups0 ? first + j - groups0 : first + j) * kGroupRows + side;
+            const uint16_t* x = t.x + b * t.batch + s * t.token + head * t.head + 8 * c16;
 #pragma unroll
-        for (int i = 0; i < kGroupRows; i += 2) {
-            const int row = g + i + side, h = first + row;
-            if (row < rows) copy16(mine + row * 256 + 16 * c16, h < q_heads ? xq + h * a.src[0].head : xk + (h - q_heads) * a.src[1].head);
+            for (int i = 0; i < kGroupRows; i += 2, x += 2 * t.head)
+                if (head + i < t.heads) copy16(mine + (j * kGroupRows + i + side) * 256 + 16 * c16, x);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-
     stage_pairs(a.angles, pairs);
-    if (kNorm) {
-        for (int i = threadIdx.x; i < 2 * kDim; i += 32 * kUnitWarps) {
-            const float* weight = a.src[i / kDim].weight;
-            weights[i / kDim][i % kDim] = weight != nullptr ? __ldg(weight + i % kDim) : 1.0f;
-        }
-    }
     __syncthreads();
-    if (rows == 0) return;
+    if (count == 0) return;
     // Either half of the warp computes two of a lane's four angles.
     float cs[4], sn[4];
 #pragma unroll
@@ -280,15 +275,22 @@ __global__ void __launch_bounds__(32 * kUnitWarps, 7) rotary_kernel(const __grid
         sn[i] = side ? s : t.y, sn[2 + i] = side ? t.y : s;
     }
     const Turns turns = make_turns(make_float4(cs[0], cs[1], cs[2], cs[3]), make_float4(sn[0], sn[1], sn[2], sn[3]));
-    uint16_t* const yq = static_cast<uint16_t*>(a.src[0].y) + token * q_heads * kDim;
-    uint16_t* const yk = static_cast<uint16_t*>(a.src[1].y) + token * a.src[1].heads * kDim;
 
-    const auto group = [&](int g) {
+    for (int j = 0; j < count; ++j) {
+        // Every warp has four groups of copies, the last ones empty where it has fewer; those behind j may be under way.
+        // Lanes read what other lanes copied, hence the __syncwarp.
+        if (j == 0) wait_copies<3>();
+        else if (j == 1) wait_copies<2>();
+        else if (j == 2) wait_copies<1>();
+        else wait_copies<0>();
+        __syncwarp();
+        const Source& t = a.src[first + j >= groups0];
+        const int head = (first + j >= groups0 ? first + j - groups0 : first + j) * kGroupRows + side;
         constexpr int kRows = kGroupRows / 2;
         Four v[kRows];
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const uint8_t* from = mine + min(g + 2 * i + side, rows - 1) * 256;
+        for (int i = 0; i < kRows; ++i) {  // (what lies behind the last head is computed on, and not stored)
+            const uint8_t* from = mine + (j * kGroupRows + 2 * i + side) * 256;
             uint4 raw;
             if (kHalf) {
                 const uint2 lo = *reinterpret_cast<const uint2*>(from + 8 * c16), hi = *reinterpret_cast<const uint2*>(from + 8 * c16 + 128);
@@ -298,53 +300,34 @@ __global__ void __launch_bounds__(32 * kUnitWarps, 7) rotary_kernel(const __grid
             }
             v[i] = widen_pairs<DT, kHalf>(raw);
         }
-        float r[kRows];
-        if (kNorm) norm_factors<kRows>(v, a.angles.eps, c16, r);
+        if (kNorm && t.weight != nullptr) {
+            const Four w = load_weights<kHalf>(t.weight, c16);
+            float r[kRows];
+            norm_factors<kRows>(v, a.angles.eps, c16, r);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const uint64_t r2 = pack2(r[i], r[i]);
+                times(v[i], Four{{r2, r2}, {r2, r2}});
+                times(v[i], w);
+            }
+        }
+        uint16_t* const y = static_cast<uint16_t*>(t.y) + (token * t.heads + head) * kDim + (kHalf ? 4 : 8) * c16;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int row = g + 2 * i + side, h = first + row;
-            if (kNorm) {
-                // (A tensor without weights is multiplied by 1 and 1.)
-                const float k = a.src[h < q_heads ? 0 : 1].weight != nullptr ? r[i] : 1.0f;
-                const uint64_t k2 = pack2(k, k);
-                times(v[i], Four{{k2, k2}, {k2, k2}});
-                times(v[i], load_weights<kHalf>(weights[h < q_heads ? 0 : 1], c16));
-            }
             turn(v[i], turns);
             float f[8];
             in_order<kHalf>(v[i], f);
             const uint2 lo = make_uint2(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]));
             const uint2 hi = make_uint2(narrow2<DT>(f[4], f[5]), narrow2<DT>(f[6], f[7]));
-            uint16_t* to = h < q_heads ? yq + h * kDim : yk + (h - q_heads) * kDim;
-            if (row < rows) {
+            if (head + 2 * i < t.heads) {
                 if (kHalf) {
-                    *reinterpret_cast<uint2*>(to + 4 * c16) = lo;
-                    *reinterpret_cast<uint2*>(to + 4 * c16 + 64) = hi;
+                    *reinterpret_cast<uint2*>(y + 2 * i * kDim) = lo;
+                    *reinterpret_cast<uint2*>(y + 2 * i * kDim + 64) = hi;
                 } else {
-                    *reinterpret_cast<uint4*>(to + 8 * c16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    *reinterpret_cast<uint4*>(y + 2 * i * kDim) = make_uint4(lo.x, lo.y, hi.x, hi.y);
                 }
             }
         }
-    };
-    // (Every warp has four groups of copies, the last ones empty where it has fewer heads.  Lanes read what other lanes
-    // copied, hence the __syncwarp.)
-    wait_copies<3>();
-    __syncwarp();
-    group(0);
-    if (rows > 8) {
-        wait_copies<2>();
-        __syncwarp();
-        group(8);
-    }
-    if (rows > 16) {
-        wait_copies<1>();
-        __syncwarp();
-        group(16);
-    }
-    if (rows > 24) {
-        wait_copies<0>();
-        __syncwarp();
-        group(24);
     }
 }
 
@@ -501,19 +484,19 @@ extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void
         !take_source(k, k_out, rotary->k_weight, k_strides, Hk, 15, &a.src[1]))
         return OVC_ERR_ARGUMENT;
     a.S = S, a.tokens = B * S;
-    // A warp takes up to 32 heads, fewer where that would leave SMs without a few warps each.
-    const int64_t rows = Hq + Hk, share = a.tokens * rows / (8 * 148);
-    int64_t unit_rows = share > kUnitRows ? kUnitRows : share < 2 ? 2 : share;
-    const int64_t units = ceil_div(rows, unit_rows);
-    unit_rows = ceil_div(ceil_div(rows, units), 2) * 2;
+    // A unit has up to four groups of eight heads, fewer where that would leave SMs without a few warps each.
+    const int64_t groups = ceil_div(Hq, kGroupRows) + ceil_div(Hk, kGroupRows), share = a.tokens * groups / (8 * 148);
+    int64_t unit_groups = share > kUnitGroups ? kUnitGroups : share < 1 ? 1 : share;
+    const int64_t units = ceil_div(groups, unit_groups);
+    unit_groups = ceil_div(groups, units);
     const int64_t ctas = ceil_div(a.tokens * units, kUnitWarps);
     if (ctas > 0x7FFFFFFF) return OVC_ERR_ARGUMENT;
     const unsigned grid = static_cast<unsigned>(ctas);
-    const size_t smem = static_cast<size_t>(kUnitWarps * unit_rows * 256);
+    const size_t smem = static_cast<size_t>(kUnitWarps * unit_groups * kGroupRows * 256);
     auto s = static_cast<cudaStream_t>(stream);
     const auto launch = [&](auto bf16, auto half, auto norm) {
         rotary_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>
-            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(unit_rows), static_cast<int>(units));
+            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(units), static_cast<int>(unit_groups));
         return check_launch();
     };
     return by_variant(dtype, rotary, launch);
