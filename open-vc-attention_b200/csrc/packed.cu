@@ -119,21 +119,31 @@ __device__ __forceinline__ int warp_sum_before(int x, int lane, int* all) {
 // the longest, and the short ones fill the SMs at the end.
 template <bool kCausal>
 __device__ void find_tile(const PackedParams& p, int per_tile, int which, int lane, Item* item) {
+    constexpr int kEach = 4;  // sequences of a lane at a time: their bounds are loaded together
     int before = 0;
     bool found = false;
-    for (int base = 0; base < p.B && !found; base += 32) {
-        const int b = base + lane;
-        int q0 = 0, lq = 0;
-        if (b < p.B) bounds(p.cu_q, b, p.Tq, &q0, &lq);
-        const int n = (lq + per_tile - 1) / per_tile;
-        int all;
-        const int at = before + warp_sum_before(n, lane, &all);
-        if (which >= at && which < at + n) {
-            item->q0 = q0, item->lq = lq;
-            bounds(p.cu_k, b, p.Tk, &item->k0, &item->lk);
-            item->token0 = (n - 1 - (which - at)) * per_tile;
-            item->t0 = 0;
-            item->t1 = visible_tiles<kCausal>(lq, item->lk, item->token0, per_tile);
+    for (int base = 0; base < p.B && !found; base += 32 * kEach) {
+        const int b0 = base + kEach * lane;
+        int q0[kEach], lq[kEach], n = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            q0[i] = lq[i] = 0;
+            if (b0 + i < p.B) bounds(p.cu_q, b0 + i, p.Tq, &q0[i], &lq[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) n += (lq[i] + per_tile - 1) / per_tile;
+        int all, at = before + warp_sum_before(n, lane, &all);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int mine = (lq[i] + per_tile - 1) / per_tile;
+            if (which >= at && which < at + mine) {
+                item->q0 = q0[i], item->lq = lq[i];
+                bounds(p.cu_k, b0 + i, p.Tk, &item->k0, &item->lk);
+                item->token0 = (mine - 1 - (which - at)) * per_tile;
+                item->t0 = 0;
+                item->t1 = visible_tiles<kCausal>(lq[i], item->lk, item->token0, per_tile);
+            }
+            at += mine;
         }
         found = which < before + all;
         before += all;
@@ -837,6 +847,7 @@ struct Layout {
 };
 
 constexpr int64_t kSms = 148;
+constexpr int64_t kMostSlots = 1 << 19;  // rows of partial results: 270 MB of workspace
 
 Layout lay_out(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
     Layout l{};
@@ -845,15 +856,15 @@ Layout lay_out(int64_t B, int64_t Tq, int64_t Tk, int64_t Hq, int64_t Hk) {
     // n sequences of at least one token make at most Tq tiles, and at most one tile each that is not full.
     const auto tiles = [&](int64_t per_tile) { const int64_t t = Tq / per_tile + B; return t < Tq ? t : Tq; };
     l.mode = kWhole, l.tiles = tiles(2 * l.tokens);
-    // Split where whole row tiles leave SMs without work and there are keys enough to share.
-    const int64_t key_tiles = ceil_div(Tk, kTile);
-    if (l.tiles * Hk < kSms && l.tiles <= kMaxTiles && key_tiles >= 4 * B) {
-        l.mode = kSplitWide;
-        if (Tq * G <= kTile * B && tiles(l.tokens) <= kMaxTiles) l.mode = kSplitNarrow, l.tiles = tiles(l.tokens);
-        l.segments = kSms + l.tiles * Hk;
-        const int64_t rows = Tq * G;
-        l.slot_rows = static_cast<int>(rows < kTile ? rows : kTile);
-    }
+    const int64_t key_tiles = ceil_div(Tk, kTile), rows = Tq * G;
+    l.slot_rows = static_cast<int>(rows < kTile ? rows : kTile);
+    // Narrow where a sequence has on average no more rows than one tile, however many sequences there are: the time goes into
+    // reading keys, which two stages on alternate key tiles do faster than one, in equal shares.
+    const int64_t narrow = tiles(l.tokens), slots = (kSms + narrow * Hk) * 2 * l.slot_rows;
+    if (rows <= kTile * B && narrow <= kMaxTiles && key_tiles >= 2 * B && slots <= kMostSlots) l.mode = kSplitNarrow, l.tiles = narrow;
+    // Wide where whole row tiles leave SMs without work and there are keys enough to share.
+    else if (l.tiles * Hk < kSms && l.tiles <= kMaxTiles && key_tiles >= 4 * B) l.mode = kSplitWide;
+    l.segments = l.mode == kWhole ? 0 : kSms + l.tiles * Hk;
     return l;
 }
 

@@ -110,6 +110,19 @@ def raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_capabilities = {}
+
+
+def capability(device):
+    """torch.cuda.get_device_capability, asked for once per device."""
+    have = _capabilities.get(device.index)
+    if have is None:
+        import torch
+
+        have = _capabilities[device.index] = torch.cuda.get_device_capability(device)
+    return have
+
+
 class on_device:
     """Makes ``device`` current for a with block; costs nothing where it is current already."""
 

@@ -8,6 +8,7 @@ from dataclasses import dataclass
 
 import torch
 
+from . import _lib
 from ._dispatch import DEFAULT_MID_WINDOW_BLOCKS, DEFAULT_VERSION, require_version
 
 
@@ -42,7 +43,7 @@ def validate_qkv(q, k, v, *, floating=True):
     if q.dtype not in allowed or any(t.dtype != q.dtype for t in (k, v)):
         raise ValueError(f"Expected matching dtypes from {allowed}")
     # The reference also admits SM103 (api.py:43-44); libovc.so holds sm_100a code only.
-    if torch.cuda.get_device_capability(q.device) != (10, 0):
+    if _lib.capability(q.device) != (10, 0):
         raise ValueError("This release validates Blackwell SM100 (B200) only")
 
 
@@ -94,7 +95,7 @@ def _fused_preparation_eligible(q, k, v, *, version, mode, causal, return_lse):
         and q.shape == k.shape == v.shape
         and q.shape[-3] >= 32768
         and all(t.is_contiguous() for t in (q, k, v))
-        and torch.cuda.get_device_capability(q.device) == (10, 0)
+        and _lib.capability(q.device) == (10, 0)
         and _packed_dsl_available()
     )
 
@@ -116,7 +117,7 @@ def prepare_fp8(q, k, v, *, rotary=None):
         _check_rotary(rotary, q, k)
     from .quantization import fp8_quantize_per_block, fp8_quantize_per_head
 
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q.device):
         q, k, v, layout, shape = _layout(q, k, v)
         if rotary is not None:
             from .rotary import prepare_rotary

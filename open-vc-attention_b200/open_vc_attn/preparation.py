@@ -23,7 +23,7 @@ def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
         raise ValueError("Fused preparation requires single-sequence [S,H,128] self-attention")
     if q.shape[-3] < 32768 or any(not t.is_contiguous() for t in (q, k, v)):
         raise ValueError("Fused preparation requires contiguous Q/K/V and S >= 32768")
-    if torch.cuda.get_device_capability(q.device) != (10, 0):
+    if _lib.capability(q.device) != (10, 0):
         raise ValueError("Fused preparation is currently validated for B200 only")
     if rotary is not None:
         from .rotary import RotaryPlan
@@ -47,7 +47,7 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
 
     s, h, d = q.shape
     lib = _lib.load()
-    with torch.cuda.device(q.device):
+    with _lib.on_device(q.device):
         if cu_seqlens is None:
             cu_seqlens = torch.arange(0, s + 1, s, device=q.device, dtype=torch.int32)
         blocks = (s + 127) // 128
@@ -59,7 +59,7 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
         packed = torch.empty((h, d, padded), dtype=torch.float8_e4m3fn, device=q.device)
         amax = torch.empty((1, h), dtype=torch.float32, device=q.device)
         vs = torch.empty((1, h), dtype=torch.float32, device=q.device)
-        outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)] + [_lib.stream_pointer(q.device)]
+        outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)] + [_lib.raw_stream(q.device.index)]
         inputs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), s, h)
         if rotary is None:
             _lib.check(lib.ovc_prepare_fused(*inputs, *outputs), "ovc_prepare_fused")

@@ -296,3 +296,31 @@ def test_refusals():
     for arguments, options, match in cases:
         with pytest.raises(ValueError, match=match):
             ovc.attention_packed(*arguments, **options)
+
+
+@pytest.mark.parametrize("lengths", ["rows and keys", "one token each"])
+def test_many_sequences(lengths):
+    """Hundreds of sequences, some empty: more than a warp looks through at a time, and more than a split launch plans for."""
+    ovc = _ovc()
+    g = torch.Generator().manual_seed(7)
+    k_lens = torch.randint(0, 300, (333,), generator=g).tolist()
+    q_lens = [1] * 333 if lengths == "one token each" else torch.randint(0, 40, (333,), generator=g).tolist()
+    for count in (333, 150, 129):
+        ql, kl = q_lens[:count], k_lens[:count]
+        q, k, v = inputs(ql, kl, 4, 2, torch.bfloat16, count)
+        out, lse = ovc.attention_packed(q, k, v, cumulative(ql), cumulative(kl), causal=True, return_lse=True)
+        _check_status()
+        close(out, lse, q, k, v, ql, kl, True)
+
+
+@pytest.mark.parametrize("count,hk,low,high", [(40, 8, 1, 3000), (100, 2, 300, 900)])
+def test_single_tokens_of_many_requests(count, hk, low, high):
+    """More row tiles than SMs, each with few rows: shares of several segments."""
+    ovc = _ovc()
+    kl = torch.randint(low, high, (count,), generator=torch.Generator().manual_seed(count)).tolist()
+    ql = [1 + i % 3 for i in range(count)]
+    q, k, v = inputs(ql, kl, 4 * hk, hk, torch.float16, count)
+    out, lse = ovc.attention_packed(q, k, v, cumulative(ql), cumulative(kl), causal=True, return_lse=True)
+    _check_status()
+    close(out, lse, q, k, v, ql, kl, True)
+    assert torch.equal(out, ovc.attention_packed(q, k, v, cumulative(ql), cumulative(kl), causal=True))
