@@ -13,16 +13,27 @@
 //   stages of the whole form; narrow split (at most one tile of rows per sequence) gives both stages the same rows and every
 //   other key tile, since with one tile of rows the time goes into reading keys.
 //
-// Warp roles (384 threads): warps 0-3 / 4-7 softmax of stage 0 / 1, warp 8 TMA loads, warp 9 the products, warps 10 and
-// 11 clear the CTA's share of the rows behind the last sequence, where asked to.  Warp 8 also
-// clears the rows of a value tile behind the end of its sequence (another sequence's values may be infinite or NaN, and
-// 0 times those is NaN).
+// Warp roles (384 threads): warps 0-3 / 4-7 softmax of stage 0 / 1, warp 8 TMA loads, warp 9 the products, warps 10 and 11
+// clear the CTA's share of the rows behind the last sequence, where asked to.  Warp 8 also clears the rows of a value tile
+// behind the end of its sequence (another sequence's values may be infinite or NaN, and 0 times those is NaN).
 //
 // Tensor memory (512 columns): S0 0..127, S1 128..255, O0 256..383, O1 384..511.  The probabilities of a stage overwrite the
-// first 64 columns of its scores; the products of one thread run in the order of their issue, so S(n+1), issued behind
-// O += P(n) V(n), cannot overtake the reads of P(n), and a stage that sees S(n+1) knows O to be complete up to n.
+// first 64 columns of its scores: there is room for nothing else.  The SM's one tensor pipe runs the products of the issuing
+// thread in the order of their issue, so S(n+1), issued behind O += P(n) V(n), cannot overtake the reads of P(n), and a
+// stage that sees S(n+1) knows O to be complete up to n.
 //
 // Shared memory: Q 2 x 32 KB, a ring of five 32 KB tiles that holds K and V alternately.
+//
+// What bounds it.  Whole: a step (both stages, one key tile) is 2048 cycles of tensor pipe and as many of exponentials (128 x
+// 128 x 2 at 16 a cycle); it takes about 3300.  A stage's step is a chain - scores read and their maximum found (350 cycles),
+// two halves of exponentials (512 each and what the other stage takes of the unit), P V, Q K^T of the next tile (1120), a
+// few hand-overs of 100 to 200 - and the two stages' chains interleave.  [32768, 8, 128]: 3.6 ms in a row (1.2 PFLOP/s at the
+// power limit, where the library's matrix product reaches 1.4), 3.3 ms alone.  Tried on it, each right and slower: a warp
+// for the products of each stage (they drift into step: 1.25 times the time), two threads to a row (1.13), part of the
+// exponentials as polynomials on the FMA pipe (1.05 for an eighth to 1.3 for half: a pair costs 25 cycles of issue there and
+// 16 on the special-function unit), the exponentials started with the maximum of the tile before (1.04), a relay that
+// tells the issuing warp of landed tiles (1.03), CTAs that stay and take one row tile after another (1.03).
+// Split, narrow: the rate at which keys are read; 81 us of kernel for 487 MB (6.0 TB/s), 7.2 TB/s once under way.
 
 #include <atomic>
 
@@ -312,8 +323,8 @@ __device__ __forceinline__ float max128_nan(const uint32_t (&s)[128]) {
 }
 
 // Four lanes that hold four 16-byte pieces each of rows of their own exchange them: lane r of the four gets piece r of
-// every row, so that a store covers 64 bytes of eight rows and not 16 bytes of thirty-two (the output of 128 rows then
-// takes a quarter of the time: the store unit works through the rows of an instruction one by one).
+// every row, so that a store covers 64 bytes of eight rows and not 16 bytes of thirty-two, which the store unit works
+// through one by one (5500 cycles for the output of an item; prompts of 5000 to 1 tokens 354 -> 348 us).
 __device__ __forceinline__ void exchange4(uint4 (&u)[4], int lane) {
     const auto swap = [](uint4& keep_low, uint4& keep_high, bool high, int mask) {
         uint4 give = high ? keep_low : keep_high;
@@ -496,7 +507,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             } else if (warp == 9 && run) {
                 // ---------------- products ----------------
                 // One warp issues for both stages, in a fixed order, which keeps them half a step apart (with a warp for each
-                // stage they drifted into step: 1.25 times the time).  The issuing lane is held until all but the last
+                // stage they drift into step: 1.25 times the time).  The issuing lane is held until all but the last
                 // products have run, so what lies between two issues is kept short: slots and descriptors are carried along,
                 // the copies are waited for by the first stage that needs them (in the narrow form, where keys are what is
                 // waited for, K of the next step only once V's slot is on its way back).
