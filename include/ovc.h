@@ -290,7 +290,8 @@ int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dt
  *   cu_seqlens_q, cu_seqlens_k [B+1] int32 on the DEVICE, 0 first, not decreasing.  Lengths may be zero.  Values outside
  *       [0, T] or out of order give wrong rows but no access outside the tensors.
  *   flags: OVC_ATTN_CAUSAL: token t of lq sees the keys below t + 1 + lk - lq; OVC_ATTN_ZERO_TAIL.
- *   out [Tq,Hq,128] dense.  A row that sees no key is zero.  Rows behind the last sequence stay as they were unless
+ *   softmax_scale: > 0, and finite times log2(e) as well.
+ *   out [Tq,Hq,128] dense, not overlapping q, k or v.  A row that sees no key is zero.  Rows behind the last sequence stay as they were unless
  *       OVC_ATTN_ZERO_TAIL is given.
  *   lse [Hq,Tq] f32 or NULL: natural logarithm of the sum of exponentials of the scaled scores, -inf for a row that
  *       sees no key.

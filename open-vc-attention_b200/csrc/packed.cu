@@ -905,7 +905,7 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
                                     float* lse, void* workspace, uint32_t* status, uint32_t* host_status, void* stream) {
     if (bad_sizes(B, Tq, Tk, Hq, Hk) || !q || !k || !v || !q_strides || !k_strides || !v_strides || !cu_seqlens_q || !cu_seqlens_k || !out ||
         (dtype != OVC_F16 && dtype != OVC_BF16) || (flags & ~(OVC_ATTN_CAUSAL | OVC_ATTN_ZERO_TAIL)) != 0 || !(softmax_scale > 0.0f) ||
-        !isfinite(softmax_scale) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
+        !isfinite(softmax_scale * 1.4426950408889634f) || !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
         ((reinterpret_cast<uintptr_t>(cu_seqlens_q) | reinterpret_cast<uintptr_t>(cu_seqlens_k) | reinterpret_cast<uintptr_t>(lse)) & 3u))
         return OVC_ERR_ARGUMENT;
     for (const int64_t* s : {q_strides, k_strides, v_strides})

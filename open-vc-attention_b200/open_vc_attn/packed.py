@@ -15,6 +15,23 @@ from . import _lib
 from .forward import _raise_if_flagged, _status
 
 
+# softmax_scale, and its product with log2(e), as normal float32 numbers
+_SMALLEST_SCALE, _LARGEST_SCALE = 2.0 ** -126, 2.0 ** 127
+
+
+def _span(t):
+    begin = t.data_ptr()
+    return begin, begin + 2 * (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1)
+
+
+def _overlap(a, b):
+    """Whether the 16-bit tensors reach into each other's memory; one that lies in gaps of the other counts, too."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
 def _in_place(t):
     """(pointer, C array of the elements from one token and one head of [T,H,128] to the next); None where the rows cannot be
     read in place."""
@@ -50,8 +67,8 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     cu_seqlens_k  the same for K and V; None: that of Q.  Lengths may be zero.
     causal        token t of lq sees the keys below t + 1 + lk - lq (the last token sees every key).
     softmax_scale 1 / sqrt(128) by default.
-    out           written and returned if given ([Tq,Hq,128] contiguous, Q's type): rows behind the last sequence stay as they
-                  were.  Without it those rows of the new tensor are zero.
+    out           written and returned if given ([Tq,Hq,128] contiguous, Q's type, no memory of Q, K or V): rows behind the
+                  last sequence stay as they were.  Without it those rows of the new tensor are zero.
 
     Returns out, or (out, lse) with lse [Hq,Tq] float32, the logarithm of the sum of exponentials of the scaled scores.  A
     row that sees no key is zero, its lse -inf.  Keys of other sequences, of the padding and of the masked future never
@@ -89,13 +106,17 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
         raise ValueError("cu_seqlens_q and cu_seqlens_k must describe the same number of sequences")
     if softmax_scale is None:
         softmax_scale = 128 ** -0.5
-    if not math.isfinite(softmax_scale) or softmax_scale <= 0.0:
-        raise ValueError("softmax_scale must be positive and finite")
+    if not _SMALLEST_SCALE <= softmax_scale <= _LARGEST_SCALE:
+        raise ValueError("softmax_scale must be positive and finite, in float32 and times log2(e) as well")
     flags = _lib.OVC_ATTN_CAUSAL if causal else 0
     if out is None:
         flags |= _lib.OVC_ATTN_ZERO_TAIL
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != device or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of Q's shape, type and device")
+    elif out.requires_grad:
+        raise ValueError("Forward inference only; detach inputs explicitly")
+    elif any(_overlap(out, t) for t in (q, k, v)):
+        raise ValueError("out must not share memory with Q/K/V")
     lib = _lib.load()
     _raise_if_flagged(device)
     with _lib.on_device(device):

@@ -52,14 +52,15 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
     """Lay out a rotation for tokens at ``positions``.
 
     positions    [S, A], or [B, S, A] for a batch with positions of its own: CUDA, int32, int64 or float32 (fractional
-                 positions are allowed).  ``grid_positions`` makes those of a clip.
+                 positions are allowed).  ``grid_positions`` makes those of a clip.  Contiguous ones are referred to and read by
+                 every call and replay, so that a captured step may count on in place; others are copied here.
     axes         channels of each of the A axes, in the order of the head's channels: even, 128 in all or fewer; channels
                  behind them stay as they are (interleaved pairs only).
     theta        pair i of an axis with d channels turns by theta^(-2 i / d) radians per position.  With
                  ``frequencies="head"`` i and d count over all axes together (sections of one set of frequencies).
     interleaved  a pair is two neighbouring channels; otherwise channels i and i + 64.
     q_weight, k_weight  [128] or None: RMS norm of each head of Q / K before the rotation, x * weight / sqrt(mean(x^2) + eps).
-                 Weights are taken over as float32 at this point.
+                 Weights are copied here, as float32.
 
     Two host threads or streams may use one plan at once; it is not written after this call.
     """
@@ -88,15 +89,17 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
         if w is not None:
             if tuple(w.shape) != (128,) or not w.is_floating_point() or w.device != positions.device:
                 raise ValueError(f"{name} must be a floating-point tensor of 128 values with the positions")
-            w = w.detach().float().contiguous()
-            w = w.clone() if w.data_ptr() % 16 else w
+            w = w.detach().to(torch.float32, copy=True, memory_format=torch.contiguous_format)
         weights.append(w)
     pair_axis = [a for a, d in enumerate(axes) for _ in range(d // 2)]
     if frequencies == "axis":
         exponents = [2.0 * i / d for d in axes for i in range(d // 2)]
     else:
         exponents = [2.0 * i / total for i in range(total // 2)]
-    turns = [float(theta) ** -e / (2.0 * math.pi) for e in exponents]
+    try:
+        turns = [float(theta) ** -e / (2.0 * math.pi) for e in exponents]
+    except OverflowError:
+        raise ValueError("theta is too small: its frequencies overflow") from None
     rest = 64 - len(turns)
     turns, pair_axis = turns + [0.0] * rest, pair_axis + [0] * rest
     positions = positions.contiguous()

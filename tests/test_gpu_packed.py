@@ -324,3 +324,27 @@ def test_single_tokens_of_many_requests(count, hk, low, high):
     _check_status()
     close(out, lse, q, k, v, ql, kl, True)
     assert torch.equal(out, ovc.attention_packed(q, k, v, cumulative(ql), cumulative(kl), causal=True))
+
+
+def test_refuses_an_output_that_is_no_memory_of_its_own():
+    ovc = _ovc()
+    q, k, v = inputs([8], [8], 4, 4, torch.bfloat16, 1)
+    cu = cumulative([8])
+    both = torch.empty(16, 4, 128, device=q.device, dtype=q.dtype)
+    fused = torch.empty(8, 3, 4, 128, device=q.device, dtype=q.dtype)
+    for out, arguments in ((q, (q, k, v)), (k, (q, k, v)), (v, (q, k, v)), (both[4:12], (q, both[:8], v)), (both[4:12], (q, k, both[8:])),
+                           (fused.view(24, 4, 128)[9:17], fused.unbind(1))):
+        with pytest.raises(ValueError, match="share memory"):
+            ovc.attention_packed(*arguments, cu, out=out)
+    with pytest.raises(ValueError, match="detach"):
+        ovc.attention_packed(q, k, v, cu, out=torch.empty_like(q).requires_grad_())
+    both[:8] = q  # neighbours in one allocation are no overlap
+    got = ovc.attention_packed(both[:8], k, v, cu, out=both[8:])
+    assert torch.equal(got, ovc.attention_packed(q, k, v, cu))
+
+
+@pytest.mark.parametrize("scale", [1e-40, 3e38, 1e300])
+def test_refuses_scales_that_float32_cannot_hold(scale):
+    q, k, v = inputs([8], [8], 2, 2, torch.float16, 1)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        _ovc().attention_packed(q, k, v, cumulative([8]), softmax_scale=scale)

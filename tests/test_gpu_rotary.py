@@ -241,3 +241,14 @@ def test_refusals_on_the_device():
         ovc.rotary_plan(torch.zeros(8, 3, device=DEV, dtype=torch.int32), q_weight=torch.ones(64, device=DEV))
     empty = ovc.rotary_qk(q[:0], k[:0], ovc.rotary_plan(torch.zeros(0, 3, device=DEV, dtype=torch.int32)))
     assert empty[0].shape == (0, 2, 128)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_plan_keeps_its_weights(dtype):
+    ovc = _ovc()
+    q, k, _ = inputs((40, 2, 128), (40, 2, 128), 1, torch.bfloat16)
+    weight = torch.rand(256, device=DEV).to(dtype)[::2]
+    plan = ovc.rotary_plan(torch.arange(40, device=DEV)[:, None], axes=(128,), q_weight=weight, k_weight=weight)
+    want = ovc.rotary_qk(q, k, plan)
+    weight.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(want, ovc.rotary_qk(q, k, plan)))

@@ -37,6 +37,7 @@ def test_c_entry_refuses_bad_arguments():
                    dict(hq=129, hk=1), dict(flags=2), dict(flags=8), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
                    dict(scale=float("inf")), dict(tq=(1 << 30) + 1), dict(hk=65536, hq=65536), dict(b=(1 << 20) + 1)):
         assert call(**change) == bad, change
+    assert call(scale=3e38) == bad  # finite, but not times log2(e)
     for strides in ((0, 128), (256, 0), (-256, 128), (252, 128), (256, 130)):
         for name in ("qs", "ks", "vs"):
             assert call(**{name: (ctypes.c_int64 * 2)(*strides)}) == bad, strides

@@ -94,3 +94,15 @@ def test_c_entries_refuse_bad_arguments():
     assert fused(p, p, None, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
     assert fused(p, p, p, 1, 128, 1, None, p, p, p, p, p, p, p, None) == bad
     assert fused(p, p, p, 1, 128, 1, plan(), p, p, p + 8, p, p, p, p, None) == bad
+
+
+def test_plan_refuses_frequencies_that_overflow():
+    with pytest.raises(ValueError, match="theta"):
+        _plan_on_meta(theta=5e-324)
+
+
+def _plan_on_meta(**options):
+    class Positions(torch.Tensor):  # passes for a CUDA tensor; the refusal comes before anything is read
+        is_cuda = True
+
+    return open_vc_attn.rotary_plan(torch.zeros(4, 1, dtype=torch.int32).as_subclass(Positions), axes=(128,), **options)
