@@ -20,6 +20,31 @@ inline int check_launch() {
     return OVC_OK;
 }
 
+#ifdef __CUDACC__
+// A kernel launched behind another of its stream without the gap between them: its CTAs may start as soon as all CTAs of the
+// one before have called release_next() (or have ended) and leave room.  Until wait_for_previous() it may only read what
+// neither of the two writes, and write nothing.  In a kernel launched in the ordinary way both are empty.
+// A preparation with rotation, [32768, 8, 128]: 99 -> 91 us, [1024, 2, 128]: 36 -> 34, [73397, 14, 128]: 281 -> 278.
+template <class... Parameters, class... Arguments>
+int launch_behind(void (*kernel)(Parameters...), dim3 grid, unsigned threads, cudaStream_t stream, Arguments... arguments) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid, config.blockDim = dim3(threads), config.stream = stream;
+    config.attrs = &early, config.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&config, kernel, static_cast<Parameters>(arguments)...);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        set_last_cuda_error(static_cast<int>(err));
+        return OVC_ERR_CUDA;
+    }
+    return OVC_OK;
+}
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 // The V part of the fused preparation (prep.cu): per-head max |v| into amax_ws (which an earlier kernel on the stream has
 // reset), then the cast with the packed layout.  Arguments are the callers' to check.
 int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, float* amax_ws, void* v_packed, float* v_descale,

@@ -111,9 +111,11 @@ __global__ void __launch_bounds__(256, 2) quant_block_kernel(BlockQuantArgs a, l
     }
 }
 
-// Per-(batch, head) max |v| by atomic max over non-negative float bit patterns.  grid (blocks, H, B).
+// Per-(batch, head) max |v| by atomic max over non-negative float bit patterns.  grid (blocks, H, B).  The kernel before it
+// resets amax; V is read without waiting for that.
 template <int DT>
 __global__ void __launch_bounds__(128) head_amax_kernel(const void* v, float* amax, long long S, int H) {
+    release_next();
     const int blk = blockIdx.x, head = blockIdx.y;
     const long long batch = blockIdx.z;
     const int c16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
@@ -134,6 +136,7 @@ __global__ void __launch_bounds__(128) head_amax_kernel(const void* v, float* am
         m = absmax8(f, m);
     }
     m = cta128_max(m);
+    wait_for_previous();
     if (threadIdx.x == 0) atomicMax(reinterpret_cast<int*>(amax + batch * H + head), __float_as_int(m));
 }
 
@@ -149,16 +152,17 @@ __global__ void __launch_bounds__(128) head_cast_kernel(const void* v, const flo
     const long long first = static_cast<long long>(blk) * kTile + r0;
     const uint16_t* src = static_cast<const uint16_t*>(v) + batch * S * row_pitch + head * kDim + c16 * 8;
     uint8_t* dst = codes + batch * S * row_pitch + head * kDim + c16 * 8;
-    const float amax = fmaxf(amax_in[batch * H + head], kFloor);
-    const float scale = div_full(kQMax, amax);
-    const float descale = div_full(amax, kQMax);
-    if (descale_out != nullptr && blk == 0 && threadIdx.x == 0) descale_out[batch * H + head] = descale;
     uint4 raw[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const long long row = first + 8 * i;
         raw[i] = row < S ? ld_stream(src + row * row_pitch) : make_uint4(0, 0, 0, 0);
     }
+    wait_for_previous();
+    const float amax = fmaxf(__ldcg(amax_in + batch * H + head), kFloor);
+    const float scale = div_full(kQMax, amax);
+    const float descale = div_full(amax, kQMax);
+    if (descale_out != nullptr && blk == 0 && threadIdx.x == 0) descale_out[batch * H + head] = descale;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const long long row = first + 8 * i;
@@ -227,10 +231,6 @@ __global__ void __launch_bounds__(256) cast_pack_kernel(const void* v, const flo
     const int l16 = threadIdx.x & 15, kq = threadIdx.x >> 4;
     const long long row_pitch = static_cast<long long>(H) * kDim;
     const uint16_t* src = static_cast<const uint16_t*>(v) + batch * S * row_pitch + head * kDim + l16 * 8;
-    const float amax = fmaxf(amax_in[batch * H + head], kFloor);
-    const float scale = div_full(kQMax, amax);
-    if (descale_out != nullptr && tile == 0 && threadIdx.x == 0)
-        descale_out[batch * H + head] = div_full(amax, kQMax);
     uint4 raw[8];
 #pragma unroll
     for (int gi = 0; gi < 2; ++gi)
@@ -239,6 +239,11 @@ __global__ void __launch_bounds__(256) cast_pack_kernel(const void* v, const flo
             const long long row = static_cast<long long>(tile) * kTile + 4 * (kq + 16 * gi) + i;
             raw[gi * 4 + i] = row < S ? ld_stream(src + row * row_pitch) : make_uint4(0, 0, 0, 0);
         }
+    wait_for_previous();
+    const float amax = fmaxf(__ldcg(amax_in + batch * H + head), kFloor);
+    const float scale = div_full(kQMax, amax);
+    if (descale_out != nullptr && tile == 0 && threadIdx.x == 0)
+        descale_out[batch * H + head] = div_full(amax, kQMax);
 #pragma unroll
     for (int gi = 0; gi < 2; ++gi) {
         const int group = kq + 16 * gi;
@@ -390,14 +395,12 @@ int launch_amax_cast_pack_v(const void* v, int dtype, int64_t S, int64_t H, floa
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(H), 1);
     const int h = static_cast<int>(H);
     auto s = static_cast<cudaStream_t>(stream);
-    if (dtype == OVC_BF16) {
-        head_amax_kernel<OVC_BF16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
-        cast_pack_kernel<OVC_BF16><<<grid, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
-    } else {
-        head_amax_kernel<OVC_F16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
-        cast_pack_kernel<OVC_F16><<<grid, 256, 0, s>>>(v, amax_ws, static_cast<uint8_t*>(v_packed), v_descale, S, h, S_pad);
-    }
-    return check_launch();
+    auto* packed = static_cast<uint8_t*>(v_packed);
+    const bool bf16 = dtype == OVC_BF16;
+    if (const int rc = check_launch(); rc != OVC_OK) return rc;
+    const int rc = launch_behind(bf16 ? head_amax_kernel<OVC_BF16> : head_amax_kernel<OVC_F16>, grid, 128, s, v, amax_ws, S, h);
+    if (rc != OVC_OK) return rc;
+    return launch_behind(bf16 ? cast_pack_kernel<OVC_BF16> : cast_pack_kernel<OVC_F16>, grid, 256, s, v, amax_ws, packed, v_descale, S, h, S_pad);
 }
 
 int launch_amax_cast_v(const void* v, int dtype, int64_t B, int64_t S, int64_t H, float* amax_ws, void* codes, float* v_descale,
@@ -406,14 +409,12 @@ int launch_amax_cast_v(const void* v, int dtype, int64_t B, int64_t S, int64_t H
     const int h = static_cast<int>(H);
     auto s = static_cast<cudaStream_t>(stream);
     auto* c = static_cast<uint8_t*>(codes);
-    if (dtype == OVC_BF16) {
-        head_amax_kernel<OVC_BF16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
-        head_cast_kernel<OVC_BF16, false><<<grid, 128, 0, s>>>(v, amax_ws, c, v_descale, nullptr, S, h);
-    } else {
-        head_amax_kernel<OVC_F16><<<grid, 128, 0, s>>>(v, amax_ws, S, h);
-        head_cast_kernel<OVC_F16, false><<<grid, 128, 0, s>>>(v, amax_ws, c, v_descale, nullptr, S, h);
-    }
-    return check_launch();
+    const bool bf16 = dtype == OVC_BF16;
+    if (const int rc = check_launch(); rc != OVC_OK) return rc;
+    const int rc = launch_behind(bf16 ? head_amax_kernel<OVC_BF16> : head_amax_kernel<OVC_F16>, grid, 128, s, v, amax_ws, S, h);
+    if (rc != OVC_OK) return rc;
+    return launch_behind(bf16 ? head_cast_kernel<OVC_BF16, false> : head_cast_kernel<OVC_F16, false>, grid, 128, s, v, amax_ws, c, v_descale,
+                         nullptr, S, h);
 }
 
 }  // namespace ovc

@@ -359,6 +359,7 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
     const long long block_at = (b * a.S + row0) * heads * kDim;  // inputs and codes are dense: elements before this block
     const uint32_t pitch = static_cast<uint32_t>(heads) * kDim;  // elements from token to token; 128 tokens stay below 2^32
     // The next head's values wait in shared memory, sixteen bytes of each token where the thread that copies them reads them.
+    release_next();  // the kernel behind may read V where this one leaves room
     uint8_t* const staged = reinterpret_cast<uint8_t*>(table + 2 * kTile * kPairs) + threadIdx.x * 16;
     const auto load = [&](int row) {
         const uint16_t* x = (row >= heads ? a.src[1].x + (row - heads) * kDim : a.src[0].x + row * kDim) + block_at + (kHalf ? 4 : 8) * c16;

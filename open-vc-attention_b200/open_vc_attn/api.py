@@ -29,28 +29,30 @@ def raw_forward(q, k, v, *, version=DEFAULT_VERSION, **kwargs):
 def validate_qkv(q, k, v, *, floating=True):
     if q.ndim not in (3, 4) or k.ndim != q.ndim or v.ndim != q.ndim:
         raise ValueError("Expected [S,H,128] or [B,S,H,128] Q/K/V")
-    if any(t.shape[-1] != 128 or min(t.shape) < 1 for t in (q, k, v)):
-        raise ValueError("The convenience API requires nonempty D=128 inputs")
+    for t in (q, k, v):
+        if t.shape[-1] != 128 or t.numel() < 1:
+            raise ValueError("The convenience API requires nonempty D=128 inputs")
     if k.shape != v.shape or q.shape[-2:] != k.shape[-2:]:
         raise ValueError("The convenience API requires MHA and matching K/V shapes")
     if q.ndim == 4 and q.shape[0] != k.shape[0]:
         raise ValueError("Q/K/V batch sizes must match")
-    if any(not t.is_cuda or t.device != q.device for t in (q, k, v)):
+    device = q.device
+    if not q.is_cuda or k.device != device or v.device != device:
         raise ValueError("Q/K/V must reside on the same CUDA device")
-    if any(t.requires_grad for t in (q, k, v)):
+    if q.requires_grad or k.requires_grad or v.requires_grad:
         raise ValueError("Forward inference only; detach inputs explicitly")
     allowed = (torch.float16, torch.bfloat16) if floating else (torch.float8_e4m3fn,)
-    if q.dtype not in allowed or any(t.dtype != q.dtype for t in (k, v)):
+    if q.dtype not in allowed or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"Expected matching dtypes from {allowed}")
     # The reference also admits SM103 (api.py:43-44); libovc.so holds sm_100a code only.
-    if _lib.capability(q.device) != (10, 0):
+    if _lib.capability(device) != (10, 0):
         raise ValueError("This release validates Blackwell SM100 (B200) only")
 
 
 def _layout(q, k, v):
     original_shape = tuple(q.shape)
     if q.ndim == 3 or q.shape[0] == 1:
-        q, k, v = [t.reshape(-1, t.shape[-2], t.shape[-1]).contiguous() for t in (q, k, v)]
+        q, k, v = [(t if t.ndim == 3 else t[0]).contiguous() for t in (q, k, v)]
         sq, sk = q.shape[0], k.shape[0]
         # [0, S], built on the device (one launch) so that the call stays capturable in a CUDA graph.
         cu_q = torch.arange(0, sq + 1, sq, device=q.device, dtype=torch.int32)

@@ -30,7 +30,7 @@ def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
 
         RotaryPlan.check(rotary, q, k)
     shape = tuple(q.shape)
-    q, k, v = [t.reshape(-1, t.shape[-2], t.shape[-1]) for t in (q, k, v)]
+    q, k, v = [t if t.ndim == 3 else t[0] for t in (q, k, v)]
     if cu_seqlens is not None and (
         cu_seqlens.shape != (2,)
         or cu_seqlens.dtype != torch.int32
@@ -53,12 +53,13 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
         blocks = (s + 127) // 128
         q_blocks = (blocks + 1) // 2 * 2
         padded = blocks * 128
-        q8, k8 = [torch.empty_like(q, dtype=torch.float8_e4m3fn) for _ in range(2)]
-        qs = torch.empty((1, h, q_blocks), dtype=torch.float32, device=q.device)
-        ks = torch.empty((1, h, blocks), dtype=torch.float32, device=q.device)
-        packed = torch.empty((h, d, padded), dtype=torch.float8_e4m3fn, device=q.device)
-        amax = torch.empty((1, h), dtype=torch.float32, device=q.device)
-        vs = torch.empty((1, h), dtype=torch.float32, device=q.device)
+        q8 = torch.empty_like(q, dtype=torch.float8_e4m3fn)
+        k8 = torch.empty_like(q8)
+        qs = q.new_empty((1, h, q_blocks), dtype=torch.float32)
+        ks = q.new_empty((1, h, blocks), dtype=torch.float32)
+        packed = q8.new_empty((h, d, padded))
+        amax = q.new_empty((1, h), dtype=torch.float32)
+        vs = torch.empty_like(amax)
         outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)] + [_lib.raw_stream(q.device.index)]
         inputs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), s, h)
         if rotary is None:

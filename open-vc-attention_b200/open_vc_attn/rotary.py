@@ -182,9 +182,9 @@ def prepare_rotary(q, k, v, plan):
     s, h, _ = q.shape[-3:]
     blocks = (s + 127) // 128
     codes = [torch.empty_like(t, dtype=torch.float8_e4m3fn) for t in (q, k, v)]
-    qs = torch.empty((batch, h, blocks), dtype=torch.float32, device=q.device)
+    qs = q.new_empty((batch, h, blocks), dtype=torch.float32)
     ks = torch.empty_like(qs)
-    vs = torch.empty((batch, h), dtype=torch.float32, device=q.device)
+    vs = q.new_empty((batch, h), dtype=torch.float32)
     amax = torch.empty_like(vs)
     _lib.check(
         _lib.load().ovc_prepare_rotary(

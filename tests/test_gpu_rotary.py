@@ -252,3 +252,48 @@ def test_a_plan_keeps_its_weights(dtype):
     want = ovc.rotary_qk(q, k, plan)
     weight.zero_()
     assert all(torch.equal(a, b) for a, b in zip(want, ovc.rotary_qk(q, k, plan)))
+
+
+@pytest.mark.parametrize("s,h", [(500, 3), (32769, 2)])
+def test_preparation_captured_repeated_and_on_two_streams(s, h):
+    """The kernels of a preparation start before the ones in front of them have ended; back to back on one stream, in a
+    replayed graph and on two streams at once they give what a call by itself gives."""
+    ovc = _ovc()
+    prepare = ovc.prepare_fp8_fused if s >= 32768 else ovc.prepare_fp8
+    plan = ovc.rotary_plan(torch.arange(s, device=DEV)[:, None], axes=(128,))
+    sets = []
+    for i in range(4):
+        q, k, _ = inputs((s, h, 128), (s, h, 128), 20 + i, torch.bfloat16)
+        sets.append((q, k, (k.float() * (i + 1) - 0.5 * q.float()).to(q.dtype)))
+
+    def values(p):
+        return [t.clone().view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t.clone()
+                for t in (p.q, p.k, p.v, p.q_descale, p.k_descale, p.v_descale)]
+
+    want = []
+    for qkv in sets:
+        want.append(values(prepare(*qkv, rotary=plan)))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0][5], want[1][5])
+
+    def check(got):
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for g, w in zip(got, want) for a, b in zip(values(g), w))
+
+    check([prepare(*qkv, rotary=plan) for qkv in sets])
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    torch.cuda.synchronize()
+    for i, qkv in enumerate(sets):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(prepare(*qkv, rotary=plan))
+    check(got)
+    static = [t.clone() for t in sets[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = prepare(*static, rotary=plan)
+    for qkv, w in zip(sets, want):
+        for to, t in zip(static, qkv):
+            to.copy_(t)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(values(captured), w))
