@@ -339,9 +339,9 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int unit_groups) 
 // and walks `rows_per_cta` heads of the list (heads of q, heads of k), 512 threads, four tokens of four pairs per thread, the
 // next head's values copied to shared memory (32 KB) meanwhile.  3 bytes per element (2 read, 1 written).  The norm's factor
 // of a row is not multiplied into its values but into the row's maximum and scale.
-// [73397, 14 + 14, 128]: 146 us, with norm 167 us (789 MB: 120 us at the rate of a copy); bound by its instructions, of which
-// it issues on 60 % of the cycles.  Next head in registers: 155 / 185 us.  Max |v| found on the way, instead of by the kernel
-// behind it: 17 us more in all.
+// [73397, 14 + 14, 128]: 146 us, with norm 162 us (789 MB: 120 us at the rate of a copy); with norm it issues on two of three
+// cycles.  Next head in registers: 155 / 185 us.  Max |v| found on the way, instead of by the kernel behind it: 17 us more in
+// all.
 constexpr int kQuantThreads = 512, kQuantRows = kTile * 16 / kQuantThreads, kQuantStep = kQuantThreads / 16;
 
 template <int DT, bool kHalf, bool kNorm>
@@ -356,28 +356,26 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
     const int tokens = static_cast<int>(min(static_cast<long long>(kTile), a.S - row0));
     const int heads = a.src[0].heads;
     const int first = blockIdx.y * rows_per_cta, last = min(first + rows_per_cta, 2 * heads);
-    const long long block_at = (b * a.S + row0) * heads * kDim;  // inputs and codes are dense: elements before this block
-    const uint32_t pitch = static_cast<uint32_t>(heads) * kDim;  // elements from token to token; 128 tokens stay below 2^32
+    const uint32_t pitch = static_cast<uint32_t>(heads) * kDim;  // inputs and codes are dense: elements from token to token
+    // A thread's tokens, in elements from the block's first (128 tokens stay below 2^31).  Behind the sequence's end the last
+    // token is done again: it changes no maximum and stores the same codes.
+    uint32_t at[kQuantRows];
+#pragma unroll
+    for (int i = 0; i < kQuantRows; ++i) at[i] = min(r0 + kQuantStep * i, tokens - 1) * pitch + (kHalf ? 4 : 8) * c16;
+    const long long block_at = (b * a.S + row0) * heads * kDim;
     // The next head's values wait in shared memory, sixteen bytes of each token where the thread that copies them reads them.
-    release_next();  // the kernel behind may read V where this one leaves room
     uint8_t* const staged = reinterpret_cast<uint8_t*>(table + 2 * kTile * kPairs) + threadIdx.x * 16;
     const auto load = [&](int row) {
-        const uint16_t* x = (row >= heads ? a.src[1].x + (row - heads) * kDim : a.src[0].x + row * kDim) + block_at + (kHalf ? 4 : 8) * c16;
+        const uint16_t* const x = (row >= heads ? a.src[1].x + (row - heads) * kDim : a.src[0].x + row * kDim) + block_at;
 #pragma unroll
         for (int i = 0; i < kQuantRows; ++i) {
             uint8_t* const to = staged + i * kQuantThreads * 16;
-            if (r0 + kQuantStep * i < tokens) {
-                const uint16_t* from = x + (r0 + kQuantStep * i) * pitch;
-                if (kHalf) copy8(to, from), copy8(to + 8, from + kPairs);
-                else copy16(to, from);
-            }
+            if (kHalf) copy8(to, x + at[i]), copy8(to + 8, x + at[i] + kPairs);
+            else copy16(to, x + at[i]);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // Tokens behind the sequence: zeros, which no copy touches.
-#pragma unroll
-    for (int i = 0; i < kQuantRows; ++i)
-        if (r0 + kQuantStep * i >= tokens) *reinterpret_cast<uint4*>(staged + i * kQuantThreads * 16) = make_uint4(0, 0, 0, 0);
+    release_next();  // the kernel behind may read V where this one leaves room
     load(first);
     stage_pairs(a.angles, pairs);
     __syncthreads();
@@ -436,14 +434,12 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
             float f[8];
             in_order<kHalf>(v[i], f);
             const uint32_t lo = cast4(f[0], f[1], f[2], f[3]), hi = cast4(f[4], f[5], f[6], f[7]);  // (saturates at 448)
-            if (r0 + kQuantStep * i < tokens) {
-                uint8_t* to = dst + (r0 + kQuantStep * i) * pitch;
-                if (kHalf) {
-                    *reinterpret_cast<uint32_t*>(to + 4 * c16) = lo;
-                    *reinterpret_cast<uint32_t*>(to + 4 * c16 + 64) = hi;
-                } else {
-                    *reinterpret_cast<uint2*>(to + 8 * c16) = make_uint2(lo, hi);
-                }
+            uint8_t* const to = dst + at[i];
+            if (kHalf) {
+                *reinterpret_cast<uint32_t*>(to) = lo;
+                *reinterpret_cast<uint32_t*>(to + kPairs) = hi;
+            } else {
+                *reinterpret_cast<uint2*>(to) = make_uint2(lo, hi);
             }
         }
     }
