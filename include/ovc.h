@@ -269,15 +269,16 @@ int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const 
  * rotated values are not rounded to 16 bits in between.
  *   q, k, v dense [B,S,H,128]; q8, k8, v8 the same in fp8; q_descale, k_descale [B,H,ceil(S/128)], v_descale [B,H];
  *   amax_ws [B,H] f32 scratch (holds the per-head max |v| afterwards).
+ *   cu_seqlens [2] int32 or NULL, B == 1 only: set to 0 and S, for callers that hand such bounds on.
  */
 int ovc_prepare_rotary(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t S, int64_t H,
                        const ovc_rotary* rotary, void* q8, void* k8, void* v8, float* q_descale, float* k_descale,
-                       float* v_descale, float* amax_ws, void* stream);
+                       float* v_descale, float* amax_ws, int32_t* cu_seqlens, void* stream);
 
 /* ovc_prepare_fused with rotated (and normalised) Q and K. */
 int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H,
                              const ovc_rotary* rotary, void* q8, void* k8, void* v_packed, float* q_descale,
-                             float* k_descale, float* v_descale, float* amax_ws, void* stream);
+                             float* k_descale, float* v_descale, float* amax_ws, int32_t* cu_seqlens, void* stream);
 
 /* ---- Attention over packed sequences in 16 bits ----
  *

@@ -218,6 +218,7 @@ struct RotaryArgs {
     Source src[2];
     long long S, tokens;                 // tokens = B * S
     float* amax_init;                    // rotary_quant_kernel: optional [H], set to 0
+    int32_t* bounds;                     // rotary_quant_kernel: optional [2], set to 0 and S
 };
 
 constexpr int kGroupRows = 8, kUnitGroups = 4, kUnitWarps = 4;
@@ -385,6 +386,7 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
         table[i] = t.x, table[kTile * kPairs + i] = t.y;
     }
     __syncthreads();
+    if (a.bounds != nullptr && blk == 0 && first == 0 && b == 0 && threadIdx.x < 2) a.bounds[threadIdx.x] = threadIdx.x * static_cast<int>(a.S);
     for (int row = first; row < last; ++row) {
         const Source& t = a.src[row >= heads];
         const int head = row >= heads ? row - heads : row;
@@ -521,14 +523,15 @@ extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void
 namespace {
 
 int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int64_t S, int64_t H, const ovc_rotary* rotary, void* q8,
-                        void* k8, float* q_descale, int64_t q_stride, float* k_descale, int64_t k_stride, float* amax_init, void* stream) {
+                        void* k8, float* q_descale, int64_t q_stride, float* k_descale, int64_t k_stride, float* amax_init, int32_t* bounds,
+                        void* stream) {
     const int64_t blocks = ceil_div(S, kTile);
     const int64_t strides[3] = {S * H * kDim, H * kDim, kDim};
     RotaryArgs a{};
     if (bad_shape(dtype, B, S, H, H) || !q_descale || !k_descale || q_stride < blocks || k_stride < blocks || !take_angles(rotary, &a.angles) ||
         !take_source(q, q8, rotary->q_weight, strides, H, 7, &a.src[0]) || !take_source(k, k8, rotary->k_weight, strides, H, 7, &a.src[1]))
         return OVC_ERR_ARGUMENT;
-    a.S = S, a.tokens = B * S, a.amax_init = amax_init;
+    a.S = S, a.tokens = B * S, a.amax_init = amax_init, a.bounds = bounds;
     a.src[0].descale = q_descale, a.src[0].descale_stride = q_stride;
     a.src[1].descale = k_descale, a.src[1].descale_stride = k_stride;
     // Two CTAs run per SM.  Heads per CTA: the count whose rounds of CTAs, each of its heads and the block's angles (which
@@ -563,18 +566,20 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
 
 extern "C" int ovc_prepare_rotary(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t S, int64_t H,
                                   const ovc_rotary* rotary, void* q8, void* k8, void* v8, float* q_descale, float* k_descale,
-                                  float* v_descale, float* amax_ws, void* stream) {
-    if (!v || !v8 || !v_descale || !amax_ws || !aligned16(v) || (reinterpret_cast<uintptr_t>(v8) & 7u)) return OVC_ERR_ARGUMENT;
+                                  float* v_descale, float* amax_ws, int32_t* cu_seqlens, void* stream) {
+    if (!v || !v8 || !v_descale || !amax_ws || !aligned16(v) || (reinterpret_cast<uintptr_t>(v8) & 7u) || (cu_seqlens && B != 1))
+        return OVC_ERR_ARGUMENT;
     const int64_t blocks = ceil_div(S, kTile);
-    const int rc = launch_rotary_quant(q, k, dtype, B, S, H, rotary, q8, k8, q_descale, blocks, k_descale, blocks, amax_ws, stream);
+    const int rc = launch_rotary_quant(q, k, dtype, B, S, H, rotary, q8, k8, q_descale, blocks, k_descale, blocks, amax_ws, cu_seqlens, stream);
     return rc != OVC_OK ? rc : launch_amax_cast_v(v, dtype, B, S, H, amax_ws, v8, v_descale, stream);
 }
 
 extern "C" int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dtype, int64_t S, int64_t H, const ovc_rotary* rotary,
                                         void* q8, void* k8, void* v_packed, float* q_descale, float* k_descale, float* v_descale,
-                                        float* amax_ws, void* stream) {
+                                        float* amax_ws, int32_t* cu_seqlens, void* stream) {
     if (!v || !v_packed || !v_descale || !amax_ws || !aligned16(v) || !aligned16(v_packed)) return OVC_ERR_ARGUMENT;
     const int64_t blocks = ceil_div(S, kTile);
-    const int rc = launch_rotary_quant(q, k, dtype, 1, S, H, rotary, q8, k8, q_descale, (blocks + 1) / 2 * 2, k_descale, blocks, amax_ws, stream);
+    const int rc = launch_rotary_quant(q, k, dtype, 1, S, H, rotary, q8, k8, q_descale, (blocks + 1) / 2 * 2, k_descale, blocks, amax_ws,
+                                       cu_seqlens, stream);
     return rc != OVC_OK ? rc : launch_amax_cast_pack_v(v, dtype, S, H, amax_ws, v_packed, v_descale, stream);
 }

@@ -48,8 +48,8 @@ SIGNATURES = {
     "ovc_attention_packed": (_i, [_p, _p, _p, _p, _p, _p, _i, _p, _p, _l, _l, _l, _l, _l, _i, _f, _p, _p, _p, _p, _p, _p]),
     "ovc_attention_packed_workspace": (_l, [_l, _l, _l, _l, _l]),
     "ovc_rotary_qk": (_i, [_p, _p, _p, _p, _i, _l, _l, _l, _l, _p, _p, _p, _p]),
-    "ovc_prepare_rotary": (_i, [_p, _p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
-    "ovc_prepare_fused_rotary": (_i, [_p, _p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "ovc_prepare_rotary": (_i, [_p, _p, _p, _i, _l, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
+    "ovc_prepare_fused_rotary": (_i, [_p, _p, _p, _i, _l, _l, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p]),
     "ovc_vs_assign": (_i, [_p, _p, _p, _l, _l, _l, _p]),
     "ovc_vs_accumulate": (_i, [_p, _p, _p, _p, _l, _l, _l, _p]),
     "ovc_vs_update_centers": (_i, [_p, _p, _p, _l, _l, _p]),
@@ -131,7 +131,7 @@ class on_device:
     def __init__(self, device):
         import torch
 
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+        self.guard = None if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
     def __enter__(self):
         if self.guard is not None:

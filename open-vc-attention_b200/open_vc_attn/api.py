@@ -10,6 +10,7 @@ import torch
 
 from . import _lib
 from ._dispatch import DEFAULT_MID_WINDOW_BLOCKS, DEFAULT_VERSION, require_version
+from .rotary import RotaryPlan, prepare_rotary
 
 
 def raw_forward(q, k, v, *, version=DEFAULT_VERSION, **kwargs):
@@ -49,13 +50,14 @@ def validate_qkv(q, k, v, *, floating=True):
         raise ValueError("This release validates Blackwell SM100 (B200) only")
 
 
-def _layout(q, k, v):
+def _layout(q, k, v, bounds=None):
+    """``bounds``: int32 [2] that the preparation will set to [0, S], where Q and K have the same tokens."""
     original_shape = tuple(q.shape)
     if q.ndim == 3 or q.shape[0] == 1:
         q, k, v = [(t if t.ndim == 3 else t[0]).contiguous() for t in (q, k, v)]
         sq, sk = q.shape[0], k.shape[0]
         # [0, S], built on the device (one launch) so that the call stays capturable in a CUDA graph.
-        cu_q = torch.arange(0, sq + 1, sq, device=q.device, dtype=torch.int32)
+        cu_q = torch.arange(0, sq + 1, sq, device=q.device, dtype=torch.int32) if bounds is None else bounds
         kwargs = {
             "cu_seqlens_q": cu_q,
             "cu_seqlens_k": cu_q if sk == sq else torch.arange(0, sk + 1, sk, device=q.device, dtype=torch.int32),
@@ -102,12 +104,6 @@ def _fused_preparation_eligible(q, k, v, *, version, mode, causal, return_lse):
     )
 
 
-def _check_rotary(rotary, q, k):
-    from .rotary import RotaryPlan
-
-    RotaryPlan.check(rotary, q, k)
-
-
 def prepare_fp8(q, k, v, *, rotary=None):
     """Q/K: per 128 tokens per head; V: per sequence per head; E4M3 max 448.
 
@@ -116,16 +112,15 @@ def prepare_fp8(q, k, v, *, rotary=None):
     """
     validate_qkv(q, k, v)
     if rotary is not None:
-        _check_rotary(rotary, q, k)
+        RotaryPlan.check(rotary, q, k)
+        with _lib.on_device(q.device):
+            bounds = q.new_empty(2, dtype=torch.int32) if q.ndim == 3 or q.shape[0] == 1 else None
+            q, k, v, layout, shape = _layout(q, k, v, bounds)
+            return PreparedFP8(*prepare_rotary(q, k, v, rotary, bounds), layout, shape)
     from .quantization import fp8_quantize_per_block, fp8_quantize_per_head
 
     with _lib.on_device(q.device):
         q, k, v, layout, shape = _layout(q, k, v)
-        if rotary is not None:
-            from .rotary import prepare_rotary
-
-            codes, descales = prepare_rotary(q, k, v, rotary)
-            return PreparedFP8(*codes, *descales, layout, shape)
         q8, qs = fp8_quantize_per_block(q, block_l=128)
         k8, ks = fp8_quantize_per_block(k, block_l=128)
         v8, vs = fp8_quantize_per_head(v)
@@ -209,7 +204,7 @@ def attention(
     """
     validate_qkv(q, k, v)
     if rotary is not None:
-        _check_rotary(rotary, q, k)
+        RotaryPlan.check(rotary, q, k)
     if mode not in ("bf16", "expcast"):
         raise ValueError("mode must be bf16 or expcast")
     if (mode == "bf16") != (version == "reference"):

@@ -15,6 +15,7 @@ from . import _lib
 from .forward import _raise_if_flagged, _status
 
 
+_Two = ctypes.c_int64 * 2
 # softmax_scale, and its product with log2(e), as normal float32 numbers
 _SMALLEST_SCALE, _LARGEST_SCALE = 2.0 ** -126, 2.0 ** 127
 
@@ -47,7 +48,7 @@ def _in_place(t):
         head = 128
     if token <= 0 or head <= 0 or token % 8 or head % 8:
         return None
-    return pointer, (ctypes.c_int64 * 2)(token, head)
+    return pointer, _Two(token, head)
 
 
 def _check_bounds(name, cu, device):

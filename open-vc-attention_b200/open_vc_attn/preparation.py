@@ -7,6 +7,7 @@ Host side of ovc_prepare_fused; mirrors prepare_fp8_fused of the reference
 import torch
 
 from . import _lib
+from .rotary import RotaryPlan
 
 
 def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
@@ -26,8 +27,6 @@ def prepare_fp8_fused(q, k, v, *, cu_seqlens=None, rotary=None):
     if _lib.capability(q.device) != (10, 0):
         raise ValueError("Fused preparation is currently validated for B200 only")
     if rotary is not None:
-        from .rotary import RotaryPlan
-
         RotaryPlan.check(rotary, q, k)
     shape = tuple(q.shape)
     q, k, v = [t if t.ndim == 3 else t[0] for t in (q, k, v)]
@@ -48,7 +47,10 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
     s, h, d = q.shape
     lib = _lib.load()
     with _lib.on_device(q.device):
-        if cu_seqlens is None:
+        bounds = None  # int32 [2] that the quantiser sets to [0, S] on the way
+        if cu_seqlens is None and rotary is not None:
+            cu_seqlens = bounds = q.new_empty(2, dtype=torch.int32)
+        elif cu_seqlens is None:
             cu_seqlens = torch.arange(0, s + 1, s, device=q.device, dtype=torch.int32)
         blocks = (s + 127) // 128
         q_blocks = (blocks + 1) // 2 * 2
@@ -60,12 +62,14 @@ def _prepare_packed(q, k, v, shape, cu_seqlens=None, rotary=None):
         packed = q8.new_empty((h, d, padded))
         amax = q.new_empty((1, h), dtype=torch.float32)
         vs = torch.empty_like(amax)
-        outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)] + [_lib.raw_stream(q.device.index)]
+        outputs = [t.data_ptr() for t in (q8, k8, packed, qs, ks, vs, amax)]
+        stream = _lib.raw_stream(q.device.index)
         inputs = (q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), s, h)
         if rotary is None:
-            _lib.check(lib.ovc_prepare_fused(*inputs, *outputs), "ovc_prepare_fused")
+            _lib.check(lib.ovc_prepare_fused(*inputs, *outputs, stream), "ovc_prepare_fused")
         else:
-            _lib.check(lib.ovc_prepare_fused_rotary(*inputs, rotary.arguments, *outputs), "ovc_prepare_fused_rotary")
+            outputs.append(None if bounds is None else bounds.data_ptr())
+            _lib.check(lib.ovc_prepare_fused_rotary(*inputs, rotary.arguments, *outputs, stream), "ovc_prepare_fused_rotary")
         result = packed[..., :s].movedim(-1, 0)
         layout = dict(cu_seqlens_q=cu_seqlens, cu_seqlens_k=cu_seqlens, max_seqlen_q=s, max_seqlen_k=s)
         return PreparedFP8(q8, k8, result, qs, ks, vs, layout, shape, v_prepacked=True)

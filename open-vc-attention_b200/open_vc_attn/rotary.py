@@ -15,6 +15,7 @@ import torch
 
 from . import _lib
 
+_Three = ctypes.c_int64 * 3
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
@@ -23,6 +24,7 @@ class RotaryPlan:
     """What ``rotary_plan`` laid out; kept by the caller for as long as positions and weights stay the same."""
 
     positions: torch.Tensor
+    tokens: tuple
     axes: tuple
     interleaved: bool
     q_weight: torch.Tensor
@@ -42,9 +44,9 @@ class RotaryPlan:
             raise ValueError("Rotary positions need Q and K of the same tokens")
         if self.positions.device != q.device:
             raise ValueError("Rotary positions must reside with Q and K")
-        tokens = self.positions.shape[:-1]
+        tokens = self.tokens
         if tokens != (s,) and tokens != (batch, s):
-            raise ValueError(f"Rotary positions are for {tuple(tokens)} tokens, Q and K have {(batch, s)}")
+            raise ValueError(f"Rotary positions are for {tokens} tokens, Q and K have {(batch, s)}")
 
 
 def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True, frequencies="axis", q_weight=None,
@@ -109,7 +111,7 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
         ctypes.addressof(host[1]), *[None if w is None else w.data_ptr() for w in weights], _POSITION_TYPES[positions.dtype],
         len(axes), 0 if interleaved else 1, eps,
     )
-    return RotaryPlan(positions, axes, bool(interleaved), *weights, float(eps), *host, ctypes.pointer(arguments))
+    return RotaryPlan(positions, tuple(positions.shape[:-1]), axes, bool(interleaved), *weights, float(eps), *host, ctypes.pointer(arguments))
 
 
 def grid_positions(frames, height, width, *, text=0, start=(0, 0, 0), device="cuda"):
@@ -123,16 +125,20 @@ def grid_positions(frames, height, width, *, text=0, start=(0, 0, 0), device="cu
 
 
 def _strides(t):
-    """Elements from one batch item, token and head of [S,H,128] or [B,S,H,128] to the next; None where the heads cannot be
-    read in place by 16-byte accesses."""
-    stride, shape = t.stride(), t.shape
+    """Elements from one batch item, token and head of [S,H,128] or [B,S,H,128] to the next, as a C array; None where the heads
+    cannot be read in place by 16-byte accesses."""
+    shape = t.shape
+    if t.is_contiguous():
+        token = 128 * shape[-2]
+        return None if t.data_ptr() % 16 else _Three(shape[-3] * token, token, 128)
+    stride = t.stride()
     if stride[-1] != 1 or t.data_ptr() % 16:
         return None
     # the stride of a dimension of one entry is never used, and may be anything
     used = [0 if n == 1 else s for n, s in zip(shape[:-1], stride)]
     if any(s % 8 for s in used):
         return None
-    return used if len(used) == 3 else [0, *used]
+    return _Three(*used) if len(used) == 3 else _Three(0, *used)
 
 
 def rotary_qk(q, k, plan):
@@ -154,44 +160,43 @@ def rotary_qk(q, k, plan):
     RotaryPlan.check(plan, q, k, "plan")
     lib = _lib.load()
     with _lib.on_device(device):
-        outs, arguments, keep = [], [], []
-        for t in (q, k):
-            outs.append(torch.empty_like(t, memory_format=torch.contiguous_format))
-            strides = _strides(t)
-            if strides is None:
-                t = t.clone(memory_format=torch.contiguous_format)
-                strides = [t.shape[-3] * t.shape[-2] * 128, t.shape[-2] * 128, 128]
-            keep.append(t)
-            arguments += [t.data_ptr(), (ctypes.c_int64 * 3)(*strides)]
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         if q.numel() == 0:
-            return tuple(outs)
+            return q_out, k_out
+        q_strides, k_strides = _strides(q), _strides(k)
+        if q_strides is None:
+            q = q.clone(memory_format=torch.contiguous_format)
+            q_strides = _strides(q)
+        if k_strides is None:
+            k = k.clone(memory_format=torch.contiguous_format)
+            k_strides = _strides(k)
         _lib.check(
             lib.ovc_rotary_qk(
-                *arguments, code, q.shape[0] if q.ndim == 4 else 1, q.shape[-3], q.shape[-2], k.shape[-2], plan.arguments,
-                outs[0].data_ptr(), outs[1].data_ptr(), _lib.raw_stream(device.index),
+                q.data_ptr(), q_strides, k.data_ptr(), k_strides, code, q.shape[0] if q.ndim == 4 else 1, q.shape[-3],
+                q.shape[-2], k.shape[-2], plan.arguments, q_out.data_ptr(), k_out.data_ptr(), _lib.raw_stream(device.index),
             ),
             "ovc_rotary_qk",
         )
-    return tuple(outs)
+    return q_out, k_out
 
 
-def prepare_rotary(q, k, v, plan):
+def prepare_rotary(q, k, v, plan, bounds=None):
     """fp8_quantize_per_block of rotated Q and K and fp8_quantize_per_head of V, dense inputs: codes of the inputs' shapes, and
-    (q, k, v) descales [B,H,blocks], [B,H,blocks], [B,H]."""
-    batch = q.shape[0] if q.ndim == 4 else 1
+    the descales of Q, K [B,H,blocks] and V [B,H].  ``bounds``: int32 [2] to be set to [0, S] (one sequence)."""
     s, h, _ = q.shape[-3:]
-    blocks = (s + 127) // 128
-    codes = [torch.empty_like(t, dtype=torch.float8_e4m3fn) for t in (q, k, v)]
-    qs = q.new_empty((batch, h, blocks), dtype=torch.float32)
+    batch = q.shape[0] if q.ndim == 4 else 1
+    q8, k8, v8 = [torch.empty_like(t, dtype=torch.float8_e4m3fn) for t in (q, k, v)]
+    qs = q.new_empty((batch, h, (s + 127) // 128), dtype=torch.float32)
     ks = torch.empty_like(qs)
     vs = q.new_empty((batch, h), dtype=torch.float32)
     amax = torch.empty_like(vs)
     _lib.check(
         _lib.load().ovc_prepare_rotary(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.dtype_code(q.dtype), batch, s, h, plan.arguments,
-            *[t.data_ptr() for t in codes], qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), amax.data_ptr(),
-            _lib.raw_stream(q.device.index),
+            q8.data_ptr(), k8.data_ptr(), v8.data_ptr(), qs.data_ptr(), ks.data_ptr(), vs.data_ptr(), amax.data_ptr(),
+            None if bounds is None else bounds.data_ptr(), _lib.raw_stream(q.device.index),
         ),
         "ovc_prepare_rotary",
     )
-    return codes, (qs, ks, vs)
+    return q8, k8, v8, qs, ks, vs

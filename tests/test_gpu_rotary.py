@@ -297,3 +297,21 @@ def test_preparation_captured_repeated_and_on_two_streams(s, h):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(values(captured), w))
+
+
+@pytest.mark.parametrize("s,fused", [(1, False), (300, False), (32768, True), (32900, True)])
+def test_preparation_hands_its_bounds_on(s, fused):
+    ovc = _ovc()
+    q, k, _ = inputs((s, 2, 128), (s, 2, 128), 9, torch.float16)
+    plan = ovc.rotary_plan(torch.arange(s, device=DEV)[:, None], axes=(128,))
+    for first in (q, q[None]):
+        second = k.reshape(first.shape)
+        prepared = (ovc.prepare_fp8_fused if fused else ovc.prepare_fp8)(first, second, second, rotary=plan)
+        layout = prepared.layout
+        assert layout["cu_seqlens_q"].tolist() == layout["cu_seqlens_k"].tolist() == [0, s]
+        assert layout["max_seqlen_q"] == layout["max_seqlen_k"] == s
+    if fused:
+        mine = torch.tensor([0, s], device=DEV, dtype=torch.int32)
+        assert ovc.prepare_fp8_fused(q, k, k, cu_seqlens=mine, rotary=plan).layout["cu_seqlens_q"] is mine
+    batch = ovc.prepare_fp8(torch.stack([q, k]), torch.stack([k, q]), torch.stack([k, k]), rotary=plan)
+    assert batch.layout == {}

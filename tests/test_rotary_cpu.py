@@ -85,15 +85,16 @@ def test_c_entries_refuse_bad_arguments():
     assert rotate() == bad
     turns[3] = 0.0
     general = lib.ovc_prepare_rotary
-    assert general(p, p, p, 1, 1, 128, 1, plan(), p + 4, p, p, p, p, p, p, None) == bad  # misaligned codes
-    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p + 4, p, p, p, p, None) == bad
-    assert general(p, p, p, 7, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
-    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p, p, None, p, p, None) == bad
-    assert general(p, p, p + 2, 1, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p + 4, p, p, p, p, p, p, None, None) == bad  # misaligned codes
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p + 4, p, p, p, p, None, None) == bad
+    assert general(p, p, p, 7, 1, 128, 1, plan(), p, p, p, p, p, p, p, None, None) == bad
+    assert general(p, p, p, 1, 1, 128, 1, plan(), p, p, p, p, None, p, p, None, None) == bad
+    assert general(p, p, p + 2, 1, 1, 128, 1, plan(), p, p, p, p, p, p, p, None, None) == bad
+    assert general(p, p, p, 1, 2, 128, 1, plan(), p, p, p, p, p, p, p, p, None) == bad  # bounds of a batch
     fused = lib.ovc_prepare_fused_rotary
-    assert fused(p, p, None, 1, 128, 1, plan(), p, p, p, p, p, p, p, None) == bad
-    assert fused(p, p, p, 1, 128, 1, None, p, p, p, p, p, p, p, None) == bad
-    assert fused(p, p, p, 1, 128, 1, plan(), p, p, p + 8, p, p, p, p, None) == bad
+    assert fused(p, p, None, 1, 128, 1, plan(), p, p, p, p, p, p, p, None, None) == bad
+    assert fused(p, p, p, 1, 128, 1, None, p, p, p, p, p, p, p, None, None) == bad
+    assert fused(p, p, p, 1, 128, 1, plan(), p, p, p + 8, p, p, p, p, None, None) == bad
 
 
 def test_plan_refuses_frequencies_that_overflow():
