@@ -76,7 +76,8 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     contribute, whatever they hold; values that are not finite within a row's own sequence may reach rows that do not see
     them.  Scores, sums and the accumulator are float32; probabilities are rounded to the inputs' type for the second product.
 
-    Stream ordered, no synchronisation, capturable.  As for ``attention``, a launch whose bounded waits expire leaves NaN and is
+    Stream ordered, no synchronisation, capturable (after a call outside of a capture, since the first one on a device allocates
+    a status word).  As for ``attention``, a launch whose bounded waits expire leaves NaN and is
     reported by a later call or by ``forward.check_status``.
     """
     if q.ndim != 3 or k.ndim != 3:
