@@ -45,7 +45,7 @@ extern "C" {
 #define OVC_ATTN_CAUSAL 1     /* bottom-right aligned causal mask */
 #define OVC_ATTN_V_UNPACKED 2 /* v is [B,Sk,H,128] FP8 (the layout of the quantisers' output), not the packed one */
 
-#define OVC_ATTN_ZERO_TAIL 4  /* ovc_attention_packed: rows of out behind the last sequence are set to zero */
+#define OVC_ATTN_ZERO_TAIL 4  /* ovc_attention_packed: rows of out behind the last sequence are set to zero, of lse to -inf */
 
 #define OVC_STATUS_WAIT_EXPIRED 1u /* a bounded barrier wait gave up; the output rows of that launch hold NaN */
 

@@ -72,7 +72,7 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
                   last sequence stay as they were.  Without it those rows of the new tensor are zero.
 
     Returns out, or (out, lse) with lse [Hq,Tq] float32, the logarithm of the sum of exponentials of the scaled scores.  A
-    row that sees no key is zero, its lse -inf.  Keys of other sequences, of the padding and of the masked future never
+    row that sees no key is zero, its lse -inf, and so is the lse of rows behind the last sequence.  Keys of other sequences, of the padding and of the masked future never
     contribute, whatever they hold; values that are not finite within a row's own sequence may reach rows that do not see
     them.  Scores, sums and the accumulator are float32; probabilities are rounded to the inputs' type for the second product.
 
@@ -122,9 +122,11 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
     lib = _lib.load()
     _raise_if_flagged(device)
     with _lib.on_device(device):
+        lse = None
+        if return_lse:  # (the kernel sets what lies behind the last sequence together with the rows of out only)
+            lse = q.new_empty((hq, tq), dtype=torch.float32) if out is None else q.new_full((hq, tq), -math.inf, dtype=torch.float32)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        lse = q.new_empty((hq, tq), dtype=torch.float32) if return_lse else None
         if tq == 0:
             return (out, lse) if return_lse else out
         if tk == 0:

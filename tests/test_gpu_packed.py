@@ -348,3 +348,14 @@ def test_refuses_scales_that_float32_cannot_hold(scale):
     q, k, v = inputs([8], [8], 2, 2, torch.float16, 1)
     with pytest.raises(ValueError, match="softmax_scale"):
         _ovc().attention_packed(q, k, v, cumulative([8]), softmax_scale=scale)
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [([300, 40], [300, 40]), ([1, 2], [4000, 300]), ([0, 0], [9, 0])])
+@pytest.mark.parametrize("given", [False, True])
+def test_lse_behind_the_last_sequence(q_lens, k_lens, given):
+    ovc = _ovc()
+    q, k, v = inputs(q_lens, k_lens, 4, 1, torch.float16, 6, extra=200)
+    q.new_full((4, q.shape[0]), math.nan, dtype=torch.float32)  # memory that the allocator may hand out next
+    _, lse = ovc.attention_packed(q, k, v, cumulative(q_lens), cumulative(k_lens), return_lse=True, out=torch.empty_like(q) if given else None)
+    end = sum(q_lens)
+    assert bool((lse[:, end:] == -math.inf).all()) and bool(torch.isfinite(lse[:, :end]).all())
