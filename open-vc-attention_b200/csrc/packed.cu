@@ -599,7 +599,10 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             const int my_steps = go ? steps_of<kCausal, kMode>(p, item, stage) : 0;
 
             float top = -INFINITY;     // the maximum that the accumulator is scaled by
-            float shift = 0.0f;        // -top * scale_log2, 0 while there is no maximum
+            // Probabilities of fp16 are 2^7 times as large, so that what its exponents cannot hold is below 2^-32 of the row's
+            // largest (2^-25 without; with hundreds of thousands of small ones that would be per cents of the row).
+            constexpr float kLift = kBf16 ? 0.0f : 7.0f;
+            float shift = 0.0f;        // kLift - top * scale_log2, 0 while there is no maximum
             float limit = -INFINITY;   // a scaled score above it moves the maximum
             // Steps whose tile every row of the warp sees in full.
             const int whole_tiles = static_cast<int>(__reduce_min_sync(0xFFFFFFFFu, static_cast<unsigned>(keys))) / kTile - item.t0;
@@ -623,17 +626,17 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         if (c >= columns) s[c] = 0xFF800000u;  // -inf, whatever the key holds
                 }
                 // The maximum moves only when it grows by more than 2^8: until then probabilities above 1 are as exact as those
-                // below, and neither the sums (float32) nor the 16-bit probabilities (up to 256) come near an overflow.  The
+                // below, and neither the sums (float32) nor the 16-bit probabilities (up to 2^15) overflow.  The
                 // comparison is false where both are -inf (no key yet) and true where a score is not a number.
                 const float tile_top = max128_nan(s);
                 if (__any_sync(0xFFFFFFFFu, !(tile_top * p.scale_log2 <= limit) && tile_top != -INFINITY)) {
                     float alpha = 1.0f;
                     if (tile_top * p.scale_log2 > limit) {
-                        alpha = ex2(fmaf(-tile_top, p.scale_log2, -shift));  // 0 for the first finite maximum
-                        if (top == -INFINITY) alpha = 0.0f;
+                        const float moved = fmaf(-tile_top, p.scale_log2, kLift);
+                        alpha = top == -INFINITY ? 0.0f : ex2(moved - shift);
                         top = tile_top;
-                        shift = -top * p.scale_log2;
-                        limit = 8.0f - shift;
+                        shift = moved;
+                        limit = 8.0f + kLift - shift;
                     }
                     if (tile_top != tile_top) alpha = nan;  // a score is not a number: neither is the row
                     float a, b;
@@ -672,11 +675,15 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         mbar_arrive(smem_addr(&sm.p_full[stage][c >> 1]));
                     }
                 }
-                // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over.
-                uint64_t part[4] = {sum2, 0, 0, 0};
+                // The sum adds the probabilities before their rounding to 16 bits (which is unbiased), behind the hand-over: a
+                // tile's first, so that many small ones are not lost one by one beside a large sum.
+                uint64_t part[4];
 #pragma unroll
-                for (int e = 0; e < 64; ++e) part[e & 3] = fadd2(part[e & 3], pack_u2(s[2 * e], s[2 * e + 1]));
-                sum2 = fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3]));
+                for (int e = 0; e < 64; ++e) {
+                    const uint64_t pair = pack_u2(s[2 * e], s[2 * e + 1]);
+                    part[e & 3] = e < 4 ? pair : fadd2(part[e & 3], pair);
+                }
+                sum2 = fadd2(sum2, fadd2(fadd2(part[0], part[1]), fadd2(part[2], part[3])));
             }
             if (ok && my_steps > 0) ok = __all_sync(0xFFFFFFFFu, wait(&sm.o_full[stage], 0));
             tc_fence_after();

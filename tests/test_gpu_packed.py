@@ -359,3 +359,26 @@ def test_lse_behind_the_last_sequence(q_lens, k_lens, given):
     _, lse = ovc.attention_packed(q, k, v, cumulative(q_lens), cumulative(k_lens), return_lse=True, out=torch.empty_like(q) if given else None)
     end = sum(q_lens)
     assert bool((lse[:, end:] == -math.inf).all()) and bool(torch.isfinite(lse[:, :end]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("split", [False, True])
+def test_many_small_probabilities_beside_a_large_one(dtype, split):
+    """One key whose probability is 2^26 times that of each of 200000 others, which hold 0.3 per cent of the row together."""
+    ovc = _ovc()
+    n, rows, h = 200000, 1 if split else 300, 8
+    q, k = [torch.zeros(t, h, 128, device=DEV, dtype=dtype) for t in (rows, n)]
+    q[..., 0], k[70000, :, 0], k[70000, :, 1] = 1.0, 18.0, 1.0
+    scale = math.log(2.0) * 26 / 18
+    v = torch.full_like(k, 1.0)
+    v[70000] = 0.0
+    out, lse = ovc.attention_packed(q, k, v, cumulative([rows]), cumulative([n]), softmax_scale=scale, return_lse=True)
+    _check_status()
+    small = (n - 1) * 2.0 ** -26
+    want = small / (1 + small)
+    # The score is exact, its product with the scale off by 2^-24 of 26 twice (scale rounded, product rounded): 2^-18 for the
+    # probabilities.  fp16 steps there are 2^-24 with the factor 2^7 or none: 2^-19 / 2^-24 is whole.  Sums of n terms: n / 8
+    # roundings at most in an accumulator of the tensor cores.  The sum of the row rounds once for a tile of 128 keys.
+    bound = 2.0 ** -18 + (n / 8) * 2.0 ** -23 + U[dtype]
+    assert bool(((out.double() - want).abs() <= bound * want).all())
+    assert bool(((lse.double() - (26 * math.log(2.0) + math.log1p(small))).abs() <= 2.0 ** -18 + 19 * 2.0 ** -24 + n / 128 * 2.0 ** -24).all())
