@@ -34,21 +34,27 @@ def _overlap(a, b):
 
 
 def _in_place(t):
-    """(pointer, C array of the elements from one token and one head of [T,H,128] to the next); None where the rows cannot be
-    read in place."""
-    token, head, channel = t.stride()
-    pointer = t.data_ptr()
-    if channel != 1 or pointer % 16:
-        return None
-    # the stride of a single token or head is never used, and may be anything
+    """Elements from one token and one head of [T,H,128] to the next, as a C array; None where the rows cannot be read in
+    place."""
     tokens, heads, _ = t.shape
+    if t.data_ptr() % 16:
+        return None
+    if t.is_contiguous():
+        return _Two(128 * heads, 128)
+    token, head, channel = t.stride()
+    # the stride of a single token or head is never used, and may be anything
     if tokens == 1:
         token = 128 * heads
     if heads == 1:
         head = 128
-    if token <= 0 or head <= 0 or token % 8 or head % 8:
+    if channel != 1 or token <= 0 or head <= 0 or token % 8 or head % 8:
         return None
-    return pointer, _Two(token, head)
+    return _Two(token, head)
+
+
+def _dense(t):
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, _in_place(t)
 
 
 def _check_bounds(name, cu, device):
@@ -137,26 +143,25 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
             else:
                 out.masked_fill_(ends[:, None, None], 0)
             return (out, lse.fill_(-math.inf)) if return_lse else out
-        arguments, keep = [], []
-        for t in (q, k, v):
-            read = _in_place(t)
-            if read is None:
-                t = t.clone(memory_format=torch.contiguous_format)
-                keep.append(t)
-                read = _in_place(t)
-            arguments += read
+        q_strides, k_strides, v_strides = _in_place(q), _in_place(k), _in_place(v)
+        if q_strides is None:
+            q, q_strides = _dense(q)
+        if k_strides is None:
+            k, k_strides = _dense(k)
+        if v_strides is None:
+            v, v_strides = _dense(v)
         sizes = (cu_seqlens_q.shape[0] - 1, tq, tk, hq, hk)
         size = lib.ovc_attention_packed_workspace(*sizes)
         workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         words, mirror = _status(device)
         _lib.check(
             lib.ovc_attention_packed(
-                *arguments, _lib.OVC_BF16 if q.dtype == torch.bfloat16 else _lib.OVC_F16, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), *sizes, flags,
-                softmax_scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
+                q.data_ptr(), q_strides, k.data_ptr(), k_strides, v.data_ptr(), v_strides,
+                _lib.OVC_BF16 if q.dtype == torch.bfloat16 else _lib.OVC_F16, cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(),
+                *sizes, flags, softmax_scale, out.data_ptr(), None if lse is None else lse.data_ptr(),
                 None if workspace is None else workspace.data_ptr(), words.data_ptr() + 4, mirror.data_ptr(),
                 _lib.raw_stream(device.index),
             ),
             "ovc_attention_packed",
         )
-        del keep, workspace
     return (out, lse) if return_lse else out
