@@ -140,13 +140,14 @@ __global__ void __launch_bounds__(128) head_amax_kernel(const void* v, float* am
     if (threadIdx.x == 0) atomicMax(reinterpret_cast<int*>(amax + batch * H + head), __float_as_int(m));
 }
 
-// V cast with the per-(batch, head) scale, row-major output.  grid (blocks, H, B).
+// V cast with the per-(batch, head) scale, row-major output.  grid (blocks, H, B), worked off from its end: what head_amax_kernel
+// read last is still in L2.
 // With SCORE also emits the per-token squared rounding residual (score[h][s], B == 1).
 template <int DT, bool SCORE>
 __global__ void __launch_bounds__(128) head_cast_kernel(const void* v, const float* amax_in, uint8_t* codes,
                                                          float* descale_out, float* score, long long S, int H) {
-    const int blk = blockIdx.x, head = blockIdx.y;
-    const long long batch = blockIdx.z;
+    const int blk = gridDim.x - 1 - blockIdx.x, head = gridDim.y - 1 - blockIdx.y;  // backwards
+    const long long batch = gridDim.z - 1 - blockIdx.z;
     const int c16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const long long row_pitch = static_cast<long long>(H) * kDim;
     const long long first = static_cast<long long>(blk) * kTile + r0;
@@ -221,13 +222,13 @@ __device__ __forceinline__ void smem_flush(const uint32_t* words, uint8_t* packe
     }
 }
 
-// V cast + pack from 16-bit input.  grid (S_pad/128, H, B), 256 threads.
+// V cast + pack from 16-bit input.  grid (S_pad/128, H, B) from its end (as above), 256 threads.
 template <int DT>
 __global__ void __launch_bounds__(256) cast_pack_kernel(const void* v, const float* amax_in, uint8_t* packed,
                                                          float* descale_out, long long S, int H, long long S_pad) {
     __shared__ __align__(16) uint32_t words[kDim * 32];
-    const int tile = blockIdx.x, head = blockIdx.y;
-    const long long batch = blockIdx.z;
+    const int tile = gridDim.x - 1 - blockIdx.x, head = gridDim.y - 1 - blockIdx.y;  // backwards
+    const long long batch = gridDim.z - 1 - blockIdx.z;
     const int l16 = threadIdx.x & 15, kq = threadIdx.x >> 4;
     const long long row_pitch = static_cast<long long>(H) * kDim;
     const uint16_t* src = static_cast<const uint16_t*>(v) + batch * S * row_pitch + head * kDim + l16 * 8;
