@@ -768,6 +768,9 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
 // Joins the partial results of a split launch: a warp per row, four channels per lane.
 //   M = max m_i,  out = sum 2^(m_i - M) O_i / sum 2^(m_i - M) l_i,  lse = ln 2 (M + log2 of that sum).
 // A partial that saw no key has l = 0 and its O was not written.
+// Bound by the chain of its loads from L2: plan, maxima and sums (a lane each), partials.  Narrow rows have many partials, of
+// which four are asked for at once; wide rows two or three (in a row 4.9 us for 512 rows of 2 to 40 partials, 16 us for 25000
+// rows; one partial after the other, each with its own maximum and sum: 6.2 and 18).
 template <bool kBf16, bool kNarrow>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ PackedParams p) {
     const PlanTiles& plan = *p.plan;
@@ -787,34 +790,51 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Pa
     const int segments = cost > 0 ? shares.owner(from + cost - 1) - share0 + 1 : 0;
     const int segment0 = share0 + kv_head * plan.count + tile;
     const int token0 = plan.token0[tile], rows = min(per_cta, lq - token0) * p.G;
+    const int stage_rows = p.tokens * p.G;
+    const uint32_t inverse = 65536u / p.G + 1;  // r / G is r * inverse >> 16 for r < 256, G < 256
     for (int r = blockIdx.z * 8 + warp; r < rows; r += 8 * gridDim.z) {
         // Row r of the row tile is row r of its only 128-row tile, or of the second one.
-        const int stage = kNarrow ? 0 : r / (p.tokens * p.G);
-        const int slot_row = r - stage * p.tokens * p.G;
+        const int stage = !kNarrow && r >= stage_rows, slot_row = r - stage * stage_rows;
         const int parts = segments * (kNarrow ? 2 : 1);
         const auto slot = [&](int i) {
             const int segment = segment0 + (kNarrow ? i >> 1 : i), s = kNarrow ? i & 1 : stage;
             return (static_cast<long long>(segment) * 2 + s) * p.slot_rows + slot_row;
         };
-        float top = -INFINITY;
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[slot(i)].x);
+        const auto max_and_sum = [&](int i) { return i < parts ? __ldcg(p.part_ml + slot(i)) : make_float2(-INFINITY, 0.0f); };
+        const float2 mine = max_and_sum(lane);
+        float top = mine.x;
+        for (int i = 32 + lane; i < parts; i += 32) top = fmaxf(top, max_and_sum(i).x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float sum = 0.0f;
-#pragma unroll 4
-        for (int i = 0; i < parts; ++i) {
-            const long long at = slot(i);
-            const float2 ml = p.part_ml[at];
-            if (ml.y == 0.0f) continue;
-            const float w = ml.y != ml.y ? ml.y : ex2(ml.x - top);
-            const float4 o = ml.y != ml.y ? make_float4(ml.y, ml.y, ml.y, ml.y) : __ldg(reinterpret_cast<const float4*>(p.part_o) + at * 32 + lane);
-            sum = fmaf(w, ml.y, sum);
-            acc.x = fmaf(w, o.x, acc.x), acc.y = fmaf(w, o.y, acc.y), acc.z = fmaf(w, o.z, acc.z), acc.w = fmaf(w, o.w, acc.w);
+        for (int base = 0; base < parts; base += 32) {  // a lane weighs a partial, all lanes add it
+            const float2 ml = base == 0 ? mine : max_and_sum(base + lane);
+            const float weight = ml.y == 0.0f ? 0.0f : ml.y != ml.y ? ml.y : ex2(ml.x - top);
+            sum = fmaf(weight, ml.y, sum);
+            const int n = min(32, parts - base);
+            constexpr int kBatch = kNarrow ? 4 : 1;
+            for (int j = 0; j < n; j += kBatch) {
+                float w[kBatch];
+                float4 o[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    w[i] = __shfl_sync(0xFFFFFFFFu, weight, (j + i) & 31);
+                    if (j + i >= n) w[i] = 0.0f;
+                    o[i] = w[i] != 0.0f ? __ldcg(reinterpret_cast<const float4*>(p.part_o) + slot(base + j + i) * 32 + lane)
+                                        : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+                    acc.x = fmaf(w[i], o[i].x, acc.x), acc.y = fmaf(w[i], o[i].y, acc.y), acc.z = fmaf(w[i], o[i].z, acc.z), acc.w = fmaf(w[i], o[i].w, acc.w);
+            }
         }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
         const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
-        const long long t = q0 + token0 + r / p.G;
-        const int head = group0 + r % p.G;
+        const int token = static_cast<int>(r * inverse >> 16);
+        const long long t = q0 + token0 + token;
+        const int head = group0 + r - token * p.G;
         reinterpret_cast<uint2*>(p.out)[(t * p.Hq + head) * 32 + lane] =
             make_uint2(narrow2<kBf16>(acc.x * factor, acc.y * factor), narrow2<kBf16>(acc.z * factor, acc.w * factor));
         if (p.lse != nullptr && lane == 0)
