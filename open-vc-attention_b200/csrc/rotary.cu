@@ -151,6 +151,25 @@ __device__ __forceinline__ void times(Four& v, const Four& w) {
 struct Turns {
     uint64_t c[2], s[2], minus_s[2];
 };
+// The rotation and the weights of the norm in one: a' = aa a + ab b, b' = ba a + bb b.
+struct Mix {
+    uint64_t aa[2], ab[2], ba[2], bb[2];
+};
+__device__ __forceinline__ Mix make_mix(const Turns& t, const Four& w) {
+    Mix m;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        m.aa[i] = fmul2(w.a[i], t.c[i]), m.ab[i] = fmul2(w.b[i], t.minus_s[i]), m.ba[i] = fmul2(w.a[i], t.s[i]), m.bb[i] = fmul2(w.b[i], t.c[i]);
+    return m;
+}
+__device__ __forceinline__ void turn(Four& v, const Mix& t) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t a = v.a[i], b = v.b[i];
+        v.a[i] = ffma2(a, t.aa[i], fmul2(b, t.ab[i]));
+        v.b[i] = ffma2(a, t.ba[i], fmul2(b, t.bb[i]));
+    }
+}
 __device__ __forceinline__ Turns make_turns(const float4& c, const float4& s) {
     return Turns{{pack2(c.x, c.y), pack2(c.z, c.w)}, {pack2(s.x, s.y), pack2(s.z, s.w)}, {pack2(-s.x, -s.y), pack2(-s.z, -s.w)}};
 }
@@ -237,21 +256,23 @@ __device__ __forceinline__ void wait_copies() {
 
 // HBM bound: 4 bytes per element (2 read, 2 written).  The heads of a token's q and then of its k are groups of eight, a unit
 // is up to four groups of one token.  A warp asks for all heads of its unit at once, computes the token's angles meanwhile -
-// four pairs to a lane, kept in registers - and then works through the groups as they arrive, two heads side by side.
-// Measured with groups of one tensor each against heads of either in a row, which cost every head a choice of pointers and
-// weights: 122 and 143 us for [4, 8191, 24 + 24, 128] with norm (805 MB; a copy of that size takes 123 us).
+// four pairs to a lane, kept in registers - and then works through the groups as they arrive, two heads side by side.  With
+// norm, the angles are multiplied by the weights once per tensor.  [4, 8191, 24 + 24, 128] with norm, at the clock that the
+// power limit leaves after some hundred calls (1.61 GHz): 125 us (805 MB; a copy of that size takes 123 us); with the weights
+// loaded and multiplied head by head 131, and with the unit's place found by a 64-bit division 138.  (Groups of one tensor:
+// heads of either in a row, which cost every head a choice of pointers and weights, took 143 us where this took 122.)
 template <int DT, bool kHalf, bool kNorm>
 __global__ void __launch_bounds__(32 * kUnitWarps, 7)
-rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int unit_groups) {
+rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_groups) {
     extern __shared__ __align__(16) uint8_t staged[];
     __shared__ Pairs pairs;
     const int lane = threadIdx.x & 31, c16 = lane & 15, side = lane >> 4;
-    const long long unit = static_cast<long long>(blockIdx.x) * kUnitWarps + (threadIdx.x >> 5);
-    const long long wanted = unit / units, token = min(wanted, a.tokens - 1);
+    const uint32_t wanted = blockIdx.x * kUnitWarps + (threadIdx.x >> 5), tokens = static_cast<uint32_t>(a.tokens);
+    const long long token = min(wanted, tokens - 1);
     const int groups0 = (a.src[0].heads + kGroupRows - 1) / kGroupRows, all = groups0 + (a.src[1].heads + kGroupRows - 1) / kGroupRows;
-    const int first = static_cast<int>(unit - wanted * units) * unit_groups;
-    const int count = wanted < a.tokens ? min(unit_groups, all - first) : 0;
-    const long long b = token / a.S, s = token - b * a.S;
+    const int first = blockIdx.y * unit_groups;
+    const int count = wanted < tokens ? min(unit_groups, all - first) : 0;
+    const long long b = static_cast<uint32_t>(token) / static_cast<uint32_t>(a.S), s = token - b * a.S;
     uint8_t* const mine = staged + (threadIdx.x >> 5) * unit_groups * kGroupRows * 256;
 
 #pragma unroll
@@ -280,6 +301,7 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int unit_groups) 
     }
     const Turns turns = make_turns(make_float4(cs[0], cs[1], cs[2], cs[3]), make_float4(sn[0], sn[1], sn[2], sn[3]));
 
+    Mix mix;
     for (int j = 0; j < count; ++j) {
         // Every warp has four groups of copies, the last ones empty where it has fewer; those behind j may be under way.
         // Lanes read what other lanes copied, hence the __syncwarp.
@@ -305,20 +327,23 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int units, int unit_groups) 
             v[i] = widen_pairs<DT, kHalf>(raw);
         }
         if (kNorm && t.weight != nullptr) {
-            const Four w = load_weights<kHalf>(t.weight, c16);
             float r[kRows];
             norm_factors<kRows>(v, a.angles.eps, c16, r);
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
                 const uint64_t r2 = pack2(r[i], r[i]);
                 times(v[i], Four{{r2, r2}, {r2, r2}});
-                times(v[i], w);
             }
+        }
+        if (kNorm && (j == 0 || first + j == groups0)) {
+            const uint64_t one = pack2(1.0f, 1.0f);
+            mix = make_mix(turns, t.weight != nullptr ? load_weights<kHalf>(t.weight, c16) : Four{{one, one}, {one, one}});
         }
         uint16_t* const y = static_cast<uint16_t*>(t.y) + (token * t.heads + head) * kDim + (kHalf ? 4 : 8) * c16;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            turn(v[i], turns);
+            if (kNorm) turn(v[i], mix);
+            else turn(v[i], turns);
             float f[8];
             in_order<kHalf>(v[i], f);
             const uint2 lo = make_uint2(narrow2<DT>(f[0], f[1]), narrow2<DT>(f[2], f[3]));
@@ -507,14 +532,12 @@ extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void
     int64_t unit_groups = share > kUnitGroups ? kUnitGroups : share < 1 ? 1 : share;
     const int64_t units = ceil_div(groups, unit_groups);
     unit_groups = ceil_div(groups, units);
-    const int64_t ctas = ceil_div(a.tokens * units, kUnitWarps);
-    if (ctas > 0x7FFFFFFF) return OVC_ERR_ARGUMENT;
-    const unsigned grid = static_cast<unsigned>(ctas);
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, kUnitWarps)), static_cast<unsigned>(units));
     const size_t smem = static_cast<size_t>(kUnitWarps * unit_groups * kGroupRows * 256);
     auto s = static_cast<cudaStream_t>(stream);
     const auto launch = [&](auto bf16, auto half, auto norm) {
         rotary_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>
-            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(units), static_cast<int>(unit_groups));
+            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(unit_groups));
         return check_launch();
     };
     return by_variant(dtype, rotary, launch);
