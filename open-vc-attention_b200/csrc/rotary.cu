@@ -125,16 +125,6 @@ __device__ __forceinline__ Four load_weights(const float* weight, int c16) {
     else v.a[0] = pack2(x.x, x.z), v.a[1] = pack2(y.x, y.z), v.b[0] = pack2(x.y, x.w), v.b[1] = pack2(y.y, y.w);
     return v;
 }
-// This lane's eight channels of a head.
-template <bool kHalf>
-__device__ __forceinline__ uint4 load_head(const uint16_t* head, int c16) {
-    if (!kHalf) return ld_stream(head + 8 * c16);
-    uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(head + 4 * c16));
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.z), "=r"(r.w) : "l"(head + 4 * c16 + 64));
-    return r;
-}
-
 __device__ __forceinline__ float squares(const Four& v) {
     uint64_t sum = fmul2(v.a[0], v.a[0]);
     sum = ffma2(v.a[1], v.a[1], sum);
