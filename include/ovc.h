@@ -236,8 +236,8 @@ int ovc_attention_ex(const void* q8, const void* k8, const void* v_packed, const
  * No counterpart in the reference, whose callers rotate Q and K before they call it.
  *   y = turn(x * w / sqrt(mean(x^2) + eps)); each pair (a, b) of a head's channels becomes
  *   (a cos t - b sin t, a sin t + b cos t), t = 2 pi * turns[pair] * positions[token][pair_axis[pair]],
- * computed in float32 (t in float64) and rounded once.  Pair p is the channels (2p, 2p + 1), or with half_split
- * (p, p + 64); turns[p] = 0 leaves a pair unturned.  A null weight means no norm for that tensor.
+ * computed in float32 (t modulo one turn, in 64-bit fixed point) and rounded once.  Pair p is the channels (2p, 2p + 1),
+ * or with half_split (p, p + 64); turns[p] = 0 leaves a pair unturned.  A null weight means no norm for that tensor.
  */
 #define OVC_POSITIONS_I32 0
 #define OVC_POSITIONS_I64 1
@@ -246,7 +246,8 @@ int ovc_attention_ex(const void* q8, const void* k8, const void* v_packed, const
 typedef struct ovc_rotary {
     const void* positions;          /* device: [S, axes], or [B, S, axes] with position_batch_stride = S * axes */
     int64_t position_batch_stride;  /* in elements; 0: every batch item has the same positions */
-    const double* turns;            /* HOST: 64 frequencies in turns per position (read during the call) */
+    const double* turns;            /* HOST: 64 frequencies in turns per position (read during the call); of either sign,
+                                       below 2^30 in size where positions are float32 */
     const uint8_t* pair_axis;       /* HOST: 64 axis indices < axes (read during the call) */
     const float* q_weight;          /* device: [128], 16-byte aligned, or null */
     const float* k_weight;          /* device: [128], 16-byte aligned, or null */

@@ -8,8 +8,10 @@
 // Angles.  A float32 product position * frequency is off by 2^-24 of itself: 2e-3 radians at position 30000.  Only the
 // fraction of a turn counts, so a frequency is an integer in units of 2^-64 turns and the product with a position is
 // taken modulo 2^64, which drops the whole turns exactly; its upper 32 bits go to sincospif.  The angle is off by about
-// 2e-7 whatever the position, without an instruction in float64.  A token has 64 pairs, shared by all its heads;
-// everything else is float32, rounded once when it is stored.
+// 2e-7 for positions up to 2^28, without an instruction in float64; behind those the 53 bits of the frequency that a plan
+// gives count (2^-55 turns a position).  Whole turns of a frequency matter to fractional positions only, whose type carries
+// them in a second word.  A token has 64 pairs, shared by all its heads; everything else is float32, rounded once when it
+// is stored.
 //
 // A lane holds four pairs of one head and sixteen lanes a head, in both layouts of the pairs (neighbours: 16 bytes in a
 // row; halves: 8 bytes from each half of the head), so no value of a pair crosses lanes and both pair members are
@@ -34,22 +36,24 @@ struct Angles {
     long long batch_stride; // in elements; 0: the same positions for every batch item
     int type, axes;
     float eps;
-    unsigned long long turns[kPairs];  // per position, in units of 2^-64 turns; 0 leaves the pair as it is
+    unsigned long long turns[kPairs];  // per position, in units of 2^-64 turns, without the whole turns
+    int whole[kPairs];                 // the whole turns, rounded down; 0 unless the positions are float32
     uint8_t axis[kPairs];
 };
 
-// position * turns modulo one turn, in units of 2^-64, for a float32 position m * 2^e.
-__device__ __forceinline__ unsigned long long float_turns(float position, unsigned long long turns) {
+// position * (whole + turns * 2^-64) modulo one turn, in units of 2^-64, for a float32 position m * 2^e.
+__device__ __forceinline__ unsigned long long float_turns(float position, unsigned long long turns, int whole) {
     const uint32_t bits = __float_as_uint(position);
     const int field = (bits >> 23) & 255;
     if (field == 0) return 0;  // zero (a subnormal position turns nothing)
     const unsigned long long m = (bits & 0x7FFFFFu) | 0x800000u;
     const unsigned long long lo = m * turns, hi = __umul64hi(m, turns);
     const int e = field - 150;
+    const long long n = static_cast<long long>(m) * whole;  // below 2^55
     unsigned long long x;
     if (e >= 0) x = e < 64 ? lo << e : 0;
-    else if (e > -64) x = (lo >> -e) | (hi << (64 + e));
-    else x = e > -128 ? hi >> (-e - 64) : 0;
+    else if (e > -64) x = ((lo >> -e) | (hi << (64 + e))) + (static_cast<unsigned long long>(n) << (64 + e));
+    else x = (e > -128 ? hi >> (-e - 64) : 0) + static_cast<unsigned long long>(n >> min(-e - 64, 63));
     return bits >> 31 ? 0 - x : x;
 }
 
@@ -57,10 +61,12 @@ __device__ __forceinline__ unsigned long long float_turns(float position, unsign
 // a time (read from there, the angles took twice as long as everything else).
 struct Pairs {
     unsigned long long turns[kPairs];
+    int whole[kPairs];
     uint8_t axis[kPairs];
 };
 __device__ __forceinline__ void stage_pairs(const Angles& a, Pairs& pairs) {
-    if (threadIdx.x < kPairs) pairs.turns[threadIdx.x] = a.turns[threadIdx.x], pairs.axis[threadIdx.x] = a.axis[threadIdx.x];
+    const int i = threadIdx.x;
+    if (i < kPairs) pairs.turns[i] = a.turns[i], pairs.whole[i] = a.whole[i], pairs.axis[i] = a.axis[i];
 }
 
 // cos and sin of one pair at one token, whose positions start at `row`.
@@ -75,8 +81,10 @@ __device__ __forceinline__ float2 pair_turn(const Angles& a, const Pairs& pairs,
         x = static_cast<unsigned long long>(__ldg(static_cast<const long long*>(a.positions) + at)) * f;
     } else {
         const float position = __ldg(static_cast<const float*>(a.positions) + at);
-        finite = isfinite(position) || f == 0;
-        x = f == 0 ? 0 : float_turns(position, f);
+        const int whole = pairs.whole[pair];
+        const bool still = f == 0 && whole == 0;
+        finite = isfinite(position) || still;
+        x = still ? 0 : float_turns(position, f, whole);
     }
     float s, c;
     sincospif(static_cast<float>(static_cast<int>((x + 0x80000000ull) >> 32)) * 4.656612873077393e-10f, &s, &c);  // 2^-31 half turns
@@ -464,6 +472,8 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
+constexpr double kMostTurns = 1 << 30;  // per float32 position
+
 bool take_angles(const ovc_rotary* r, Angles* out) {
     if (!r || !r->positions || !r->turns || !r->pair_axis || r->axes < 1 || r->axes > 64 || !(r->eps >= 0.0f) || !isfinite(r->eps) ||
         (r->position_type != OVC_POSITIONS_I32 && r->position_type != OVC_POSITIONS_I64 && r->position_type != OVC_POSITIONS_F32) ||
@@ -473,8 +483,15 @@ bool take_angles(const ovc_rotary* r, Angles* out) {
     out->type = r->position_type, out->axes = r->axes, out->eps = r->eps;
     for (int i = 0; i < kPairs; ++i) {
         if (!isfinite(r->turns[i]) || r->pair_axis[i] >= r->axes) return false;
-        const double fraction = r->turns[i] - floor(r->turns[i]);
-        out->turns[i] = fraction < 1.0 ? static_cast<unsigned long long>(ldexp(fraction, 64)) : 0;
+        // Sign and size apart: both parts of the size are exact, and so is their negation (rounded down, a fraction above zero).
+        const bool negative = r->turns[i] < 0.0;
+        const double size = fabs(r->turns[i]), whole = floor(size);
+        const auto fraction = static_cast<unsigned long long>(ldexp(size - whole, 64));
+        out->turns[i] = negative ? 0 - fraction : fraction;
+        if (r->position_type == OVC_POSITIONS_F32) {
+            if (!(size < kMostTurns)) return false;
+            out->whole[i] = negative ? -static_cast<int>(whole) - (fraction != 0) : static_cast<int>(whole);
+        }
         out->axis[i] = r->pair_axis[i];
     }
     return true;

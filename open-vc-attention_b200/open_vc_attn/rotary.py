@@ -16,6 +16,7 @@ import torch
 from . import _lib
 
 _Three = ctypes.c_int64 * 3
+_MOST_TURNS = 2.0 ** 30  # per float32 position: the kernels carry the whole turns in 32 bits
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
 
@@ -58,8 +59,9 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
                  every call and replay, so that a captured step may count on in place; others are copied here.
     axes         channels of each of the A axes, in the order of the head's channels: even, 128 in all or fewer; channels
                  behind them stay as they are (interleaved pairs only).
-    theta        pair i of an axis with d channels turns by theta^(-2 i / d) radians per position.  With
-                 ``frequencies="head"`` i and d count over all axes together (sections of one set of frequencies).
+    theta        pair i of an axis with d channels turns by theta^(-2 i / d) radians per position (below 2^30 turns, where
+                 positions are float32).  With ``frequencies="head"`` i and d count over all axes together (sections of one
+                 set of frequencies).
     interleaved  a pair is two neighbouring channels; otherwise channels i and i + 64.
     q_weight, k_weight  [128] or None: RMS norm of each head of Q / K before the rotation, x * weight / sqrt(mean(x^2) + eps).
                  Weights are copied here, as float32.
@@ -102,6 +104,8 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
         turns = [float(theta) ** -e / (2.0 * math.pi) for e in exponents]
     except OverflowError:
         raise ValueError("theta is too small: its frequencies overflow") from None
+    if positions.dtype == torch.float32 and max(turns) >= _MOST_TURNS:
+        raise ValueError("theta is too small for fractional positions: at most 2**30 turns per position")
     rest = 64 - len(turns)
     turns, pair_axis = turns + [0.0] * rest, pair_axis + [0] * rest
     positions = positions.contiguous()

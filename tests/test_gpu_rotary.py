@@ -315,3 +315,54 @@ def test_preparation_hands_its_bounds_on(s, fused):
         assert ovc.prepare_fp8_fused(q, k, k, cu_seqlens=mine, rotary=plan).layout["cu_seqlens_q"] is mine
     batch = ovc.prepare_fp8(torch.stack([q, k]), torch.stack([k, q]), torch.stack([k, k]), rotary=plan)
     assert batch.layout == {}
+
+
+def turned(x, positions, turns, half=False):
+    """``formula`` for 64 frequencies in turns per position, of any size and sign, on one axis: the product is exact in whole
+    numbers of 2^-40 turns for the values used here, so its fraction is, too."""
+    t = (positions.double()[..., 0, None] * turns).remainder(1.0) * (2.0 * math.pi)
+    t, i = t[:, None], torch.arange(64, device=x.device)
+    at, to = (i, i + 64) if half else (2 * i, 2 * i + 1)
+    y, size = x.double(), x.double().abs()
+    a, b = x.double()[..., at], x.double()[..., to]
+    y[..., at], y[..., to] = a * t.cos() - b * t.sin(), a * t.sin() + b * t.cos()
+    size[..., at] = size[..., to] = torch.hypot(a, b)
+    return y, size
+
+
+FRACTIONAL = [0.5, 2.25, -0.5, -3.75, 0.0, 1.0, 2.0 ** -12 * 5, 4097.125, -(2.0 ** 20) + 0.5, 1.5 * 2.0 ** 30]
+
+
+@pytest.mark.parametrize("theta", [0.05, 0.1, 0.9, 1e-6, 10000.0])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_fractional_positions_and_fast_frequencies(theta, interleaved):
+    """Small thetas turn by more than a whole turn per position, of which a fractional position takes a fraction."""
+    ovc = _ovc()
+    positions = torch.tensor([p for p in FRACTIONAL if abs(p) < 5], device=DEV)[:, None]
+    s = positions.shape[0]
+    q, k, _ = inputs((s, 3, 128), (s, 2, 128), 12, torch.bfloat16)
+    got = ovc.rotary_qk(q, k, ovc.rotary_plan(positions, axes=(128,), theta=theta, interleaved=interleaved))
+    for x, y in zip((q, k), got):
+        # (below 2^20 turns in all, whose products and frequencies in 64 bits are off by 2^-31 turns at most)
+        close(y, *formula(x, positions, (128,), interleaved, theta=theta))
+
+
+@pytest.mark.parametrize("kind", [torch.float32, torch.int32, torch.int64])
+@pytest.mark.parametrize("half", [False, True])
+def test_frequencies_of_any_size_and_sign(kind, half):
+    """The C entry takes frequencies of either sign; the plan's own are replaced by some that are exact in 2^-20 turns."""
+    ovc = _ovc()
+    plan_positions = torch.tensor(FRACTIONAL, device=DEV)[:, None].to(kind)
+    s = len(FRACTIONAL)
+    plan = ovc.rotary_plan(plan_positions, axes=(128,), interleaved=not half)
+    values = [0.0, 0.25, -0.25, 1.0, -1.0, 3.0, -3.0, 1.25, -1.25, 2.0 ** -20, -(2.0 ** -20), 1023.0 + 2.0 ** -20, -1023.0 - 2.0 ** -20]
+    turns = [values[i % len(values)] for i in range(64)]
+    plan.turns[:] = turns
+    q, k, _ = inputs((s, 3, 128), (s, 2, 128), 13, torch.float16)
+    for x, y in zip((q, k), ovc.rotary_qk(q, k, plan)):
+        close(y, *turned(x, plan_positions, torch.tensor(turns, device=DEV, dtype=torch.float64), half))
+    prepared = ovc.prepare_fp8(q[:, :2].contiguous(), k, k, rotary=plan)
+    want, size = turned(k, plan_positions, torch.tensor(turns, device=DEV, dtype=torch.float64), half)
+    d = prepared.k_descale.double()[0, :, 0][None, :, None]
+    limit = (want / d).abs().mul(2.0 ** -4).clamp_min(2.0 ** -10) + 1.1 * (F32 * size / d + 4 * 2.0 ** -24 * (want / d).abs())
+    assert bool(((prepared.k.double() - want / d).abs() <= limit).all())

@@ -107,3 +107,32 @@ def _plan_on_meta(**options):
         is_cuda = True
 
     return open_vc_attn.rotary_plan(torch.zeros(4, 1, dtype=torch.int32).as_subclass(Positions), axes=(128,), **options)
+
+
+@pytest.mark.parametrize("bad", [2.0 ** 30, -(2.0 ** 30), 1e300])
+def test_c_entries_refuse_frequencies_that_fractional_positions_cannot_take(bad):
+    import __graft_entry__
+
+    __graft_entry__.build()
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096)
+    p = ctypes.addressof(buf) // 16 * 16 + 16
+    turns, axis = (ctypes.c_double * 64)(), (ctypes.c_uint8 * 64)()
+    turns[5] = bad
+    plan = _lib.OvcRotary(positions=p, position_batch_stride=0, turns=ctypes.addressof(turns), pair_axis=ctypes.addressof(axis),
+                          q_weight=None, k_weight=None, position_type=2, axes=1, half_split=0, eps=1e-6)
+    strides = (ctypes.c_int64 * 3)(1024, 256, 128)
+    assert lib.ovc_rotary_qk(p, strides, p, strides, 1, 1, 4, 2, 2, ctypes.byref(plan), p, p, None) == -1
+    assert lib.ovc_prepare_rotary(p, p, p, 1, 1, 128, 1, ctypes.byref(plan), p, p, p, p, p, p, p, None, None) == -1
+
+
+def test_plan_refuses_thetas_that_fractional_positions_cannot_take():
+    with pytest.raises(ValueError, match="fractional"):
+        _float_plan_on_meta(theta=1e-30)
+
+
+def _float_plan_on_meta(**options):
+    class Positions(torch.Tensor):
+        is_cuda = True
+
+    return open_vc_attn.rotary_plan(torch.zeros(4, 1).as_subclass(Positions), axes=(128,), **options)
