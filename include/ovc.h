@@ -293,8 +293,10 @@ int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dt
  *       [0, T] or out of order give wrong rows but no access outside the tensors.
  *   flags: OVC_ATTN_CAUSAL: token t of lq sees the keys below t + 1 + lk - lq; OVC_ATTN_ZERO_TAIL.
  *   softmax_scale: > 0, and finite times log2(e) as well.
- *   out [Tq,Hq,128] dense, not overlapping q, k or v.  A row that sees no key is zero.  Rows behind the last sequence stay as they were unless
- *       OVC_ATTN_ZERO_TAIL is given.
+ *   out [Tq,Hq,128] dense, not overlapping q, k or v.  A row that sees no key is zero, whatever v holds.  Rows behind the
+ *       last sequence stay as they were unless OVC_ATTN_ZERO_TAIL is given.  What q, k and v hold outside of a row's own
+ *       sequence never reaches it; a value of v within it that is infinite or NaN may reach a row that sees some keys, but
+ *       not that one.
  *   lse [Hq,Tq] f32 or NULL: natural logarithm of the sum of exponentials of the scaled scores, -inf for a row that
  *       sees no key.
  *   workspace: ovc_attention_packed_workspace() bytes, 16-byte aligned; NULL where that is 0.  Written before it is

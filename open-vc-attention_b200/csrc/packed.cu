@@ -693,7 +693,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
             const float sum = ok ? a + b : nan;
             if (kMode == kWhole) {
                 const bool none = top == -INFINITY && sum == sum;  // no key is visible
-                const float factor = none ? 0.0f : 1.0f / sum;
+                const float factor = 1.0f / sum;
                 const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
                 if (real && p.lse != nullptr)
                     p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
@@ -720,7 +720,8 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                         uint32_t w[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            w[i] = narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
+                            // (Zero by choice: where a value is infinite or NaN, the sum of zero times the values is NaN.)
+                            w[i] = none ? 0u : narrow2<kBf16>(__uint_as_float(o[8 * e + 2 * i]) * factor, __uint_as_float(o[8 * e + 2 * i + 1]) * factor);
                         u[e] = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     exchange4(u, lane);

@@ -78,9 +78,10 @@ def attention_packed(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, causal=False, 
                   last sequence stay as they were.  Without it those rows of the new tensor are zero.
 
     Returns out, or (out, lse) with lse [Hq,Tq] float32, the logarithm of the sum of exponentials of the scaled scores.  A
-    row that sees no key is zero, its lse -inf, and so is the lse of rows behind the last sequence.  Keys of other sequences, of the padding and of the masked future never
-    contribute, whatever they hold; values that are not finite within a row's own sequence may reach rows that do not see
-    them.  Scores, sums and the accumulator are float32; probabilities are rounded to the inputs' type for the second product.
+    row that sees no key is zero, whatever V holds, its lse -inf, and so is the lse of rows behind the last sequence.  Keys of
+    other sequences, of the padding and of the masked future never contribute, whatever they hold; values that are not finite
+    within a row's own sequence may reach rows that see some keys, but not those.  Scores, sums and the accumulator are
+    float32; probabilities are rounded to the inputs' type for the second product.
 
     Stream ordered, no synchronisation, capturable (after a call outside of a capture, since the first one on a device allocates
     a status word).  As for ``attention``, a launch whose bounded waits expire leaves NaN and is

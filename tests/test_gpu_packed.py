@@ -382,3 +382,24 @@ def test_many_small_probabilities_beside_a_large_one(dtype, split):
     bound = 2.0 ** -18 + (n / 8) * 2.0 ** -23 + U[dtype]
     assert bool(((out.double() - want).abs() <= bound * want).all())
     assert bool(((lse.double() - (26 * math.log(2.0) + math.log1p(small))).abs() <= 2.0 ** -18 + 19 * 2.0 ** -24 + n / 128 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,hk", [
+    ([300], [5], 8, 2), ([200, 700], [0, 300], 7, 1),  # whole
+    ([900], [600], 2, 2),  # wide split
+    ([40, 40, 40], [5, 20, 700], 2, 2),  # narrow split
+])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_without_keys_beside_values_that_are_not_finite(q_lens, k_lens, hq, hk, bad, dtype):
+    """Every sequence's first value is not finite: a row that sees a key sees it, a row that sees none is zero all the same."""
+    ovc = _ovc()
+    q, k, v = inputs(q_lens, k_lens, hq, hk, dtype, 17)
+    cu_q, cu_k = cumulative(q_lens), cumulative(k_lens)
+    v[cu_k[:-1].long().clamp_max(v.shape[0] - 1)] = bad
+    out, lse = ovc.attention_packed(q, k, v, cu_q, cu_k, causal=True, return_lse=True)
+    _check_status()
+    blind = torch.cat([torch.arange(a, device=DEV) + b < a for a, b in zip(q_lens, k_lens)])
+    assert bool(blind.any()) and not bool(blind.all())
+    assert not out[blind].any() and bool((lse[:, blind] == -math.inf).all())
+    assert not bool(torch.isfinite(out[~blind]).any()) and bool(torch.isfinite(lse[:, ~blind]).all())
