@@ -302,8 +302,8 @@ int ovc_prepare_fused_rotary(const void* q, const void* k, const void* v, int dt
  *   workspace: ovc_attention_packed_workspace() bytes, 16-byte aligned; NULL where that is 0.  Written before it is
  *       read; one launch at a time may use it.
  *   status: one uint32 on the device, OR-ed with OVC_STATUS_WAIT_EXPIRED by a launch whose bounded wait gave up; while it
- *       is set, launches leave NaN and return.  host_status: pinned host memory that gets the same bit.  Both or
- *       either may be NULL.
+ *       is set, launches leave NaN in out and lse and return.  host_status: pinned host memory that gets the same bit from
+ *       both.  Both or either may be NULL.
  * 1 <= Hq / Hk <= 128; Tq, Tk <= 2^30; B <= 2^20.
  */
 int ovc_attention_packed(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,

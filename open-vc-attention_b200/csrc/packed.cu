@@ -386,10 +386,16 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
     const Item& item = sm.item;
 
     if (warp == 0) {
-        // A barrier wait expired since the host last looked: start nothing, leave NaN.  (Nor could anything be computed
-        // were the tiles not on the 1024-byte grid of their swizzle.)
+        // A barrier wait expired since the host last looked: start nothing, leave NaN, and report this launch as well (the
+        // host may have taken note of the earlier one on another stream, and clears the word on its own).  (Nor could
+        // anything be computed were the tiles not on the 1024-byte grid of their swizzle.)
         if (lane == 0) {
-            sm.gave_up = (p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u) | (smem_addr(smem_raw) & 1023u);
+            const uint32_t expired = p.status != nullptr ? *reinterpret_cast<volatile uint32_t*>(p.status) : 0u;
+            if (expired != 0 && p.host_status != nullptr) {
+                *p.host_status = OVC_STATUS_WAIT_EXPIRED;
+                __threadfence_system();
+            }
+            sm.gave_up = expired | (smem_addr(smem_raw) & 1023u);
             sm.abort_flag = 0;
         }
         if (kSplit) plan_tiles<kCausal>(p, per_cta, lane, &sm.plan);
@@ -697,7 +703,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
                 const long long at = static_cast<long long>(item.q0 + token) * p.Hq + head;
                 if (real && p.lse != nullptr)
                     p.lse[static_cast<long long>(head) * p.Tq + item.q0 + token] =
-                        none || !ok ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;
+                        none ? -INFINITY : (__log2f(sum) - shift) * 0.69314718055994531f;  // (NaN where a wait expired)
                 // After the exchange a lane stores its piece of the four rows of its group.
                 uint4* to[4];
 #pragma unroll

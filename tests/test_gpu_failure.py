@@ -64,3 +64,39 @@ def test_a_failure_surfaces_at_the_next_public_call_without_a_sync():
     again = ovc.attention(q, k, v)
     forward.check_status(device)
     assert torch.equal(first, again)
+
+
+# (q lengths, k lengths, query heads, key heads) of the forms of attention_packed: whole, wide split, narrow split
+PACKED_FORMS = [([300, 40], [300, 40], 4, 2), ([300], [2000], 2, 2), ([1, 2], [4000, 300], 4, 1)]
+
+
+def _packed_inputs(q_lens, k_lens, hq, hk):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    q = torch.randn(sum(q_lens), hq, 128, generator=g, device=DEV).to(torch.bfloat16)
+    k, v = [torch.randn(sum(k_lens), hk, 128, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2)]
+    cu = [torch.tensor([0, *torch.tensor(n).cumsum(0).tolist()], dtype=torch.int32, device=DEV) for n in (q_lens, k_lens)]
+    return q, k, v, *cu
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,hk", PACKED_FORMS)
+def test_packed_launches_behind_a_failure_leave_nan_and_report_it(q_lens, k_lens, hq, hk):
+    """The sticky word is set from the host, without its mirror: as a launch finds it behind one that gave up."""
+    ovc, _lib, forward = _mods()
+    device = torch.device(DEV)
+    arguments = _packed_inputs(q_lens, k_lens, hq, hk)
+    forward.check_status(device)
+    want = ovc.attention_packed(*arguments, causal=True, return_lse=True)
+    forward.check_status(device)
+    words = forward.status_word(device)
+    words[1:].fill_(_lib.STATUS_WAIT_EXPIRED)
+    torch.cuda.synchronize()
+    out, lse = ovc.attention_packed(*arguments, causal=True, return_lse=True)
+    torch.cuda.synchronize()
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
+    words[1:].zero_()  # the launch itself has reported, whatever becomes of the word
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="bounded wait expired"):
+        ovc.attention_packed(*arguments, causal=True)
+    again = ovc.attention_packed(*arguments, causal=True, return_lse=True)
+    forward.check_status(device)
+    assert all(torch.equal(a, b) for a, b in zip(want, again))
