@@ -44,17 +44,28 @@ def _failure(value):
 
 
 def _raise_if_flagged(device):
-    """No synchronisation: looks at the host copy of the sticky word, which reflects every launch whose
-    trailing 4-byte copy has completed.  Called at the start of each public attention call."""
+    """No synchronisation unless there is a failure to report: looks at the host copy of the sticky word, which reflects every
+    launch whose trailing 4-byte copy has completed.  Called at the start of each public attention call."""
     flag = _mirrored.get(device.index)
     if flag is not None and flag.value == 0:
         return
     words, mirror = _status(device)
     value = int(mirror[0])
     if value != 0:
-        mirror.zero_()
-        words[1:].zero_()
+        _clear(device, words, mirror)
         raise _failure(value)
+
+
+def _clear(device, words, mirror):
+    """Take note of a failure.  Launches of attention_packed leave NaN while the sticky word is set, on any stream: all those
+    under way have seen it, and none that follows does.  In a capture nothing may be waited for: the next call outside of one
+    reports the failure again."""
+    if torch.cuda.is_current_stream_capturing():
+        return
+    torch.cuda.synchronize(device)
+    mirror.zero_()
+    words[1:].zero_()
+    torch.cuda.synchronize(device)
 
 
 def _publish_status(device):
@@ -66,10 +77,10 @@ def _publish_status(device):
 def check_status(device):
     """Synchronise and raise if any attention launch on ``device`` gave up on a barrier wait since the last check."""
     words, mirror = _status(device)
+    torch.cuda.synchronize(words.device)
     value = int(words[1].item())
     if value != 0:
-        words[1:].zero_()
-        mirror.zero_()
+        _clear(words.device, words, mirror)
         raise _failure(value)
 
 

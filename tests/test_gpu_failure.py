@@ -100,3 +100,52 @@ def test_packed_launches_behind_a_failure_leave_nan_and_report_it(q_lens, k_lens
     again = ovc.attention_packed(*arguments, causal=True, return_lse=True)
     forward.check_status(device)
     assert all(torch.equal(a, b) for a, b in zip(want, again))
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,hk", PACKED_FORMS)
+@pytest.mark.parametrize("by", ["call", "check_status"])
+def test_a_reported_failure_does_not_reach_another_stream(q_lens, k_lens, hq, hk, by):
+    """The failure is reported on a stream that is busy; a call on another one right behind it computes."""
+    ovc, _lib, forward = _mods()
+    device = torch.device(DEV)
+    arguments = _packed_inputs(q_lens, k_lens, hq, hk)
+    forward.check_status(device)
+    want = ovc.attention_packed(*arguments)
+    words, mirror = forward._status(device)
+    words[1:].fill_(_lib.STATUS_WAIT_EXPIRED)
+    mirror.fill_(_lib.STATUS_WAIT_EXPIRED)
+    busy, other = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(busy):
+        if by == "call":
+            torch.cuda._sleep(20_000_000)  # about 10 ms
+            with pytest.raises(RuntimeError, match="bounded wait expired"):
+                ovc.attention_packed(*arguments)
+        else:
+            with pytest.raises(RuntimeError, match="bounded wait expired"):
+                forward.check_status(device)
+    with torch.cuda.stream(other):
+        got = ovc.attention_packed(*arguments)
+    torch.cuda.synchronize()
+    assert torch.equal(want, got)
+    forward.check_status(device)
+
+
+def test_a_failure_found_in_a_capture_is_reported_again_behind_it():
+    ovc, _lib, forward = _mods()
+    device = torch.device(DEV)
+    arguments = _packed_inputs(*PACKED_FORMS[0])
+    forward.check_status(device)
+    want = ovc.attention_packed(*arguments)
+    words, mirror = forward._status(device)
+    words[1:].fill_(_lib.STATUS_WAIT_EXPIRED)
+    mirror.fill_(_lib.STATUS_WAIT_EXPIRED)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="bounded wait expired"):
+            ovc.attention_packed(*arguments)
+    with pytest.raises(RuntimeError, match="bounded wait expired"):
+        ovc.attention_packed(*arguments)
+    assert torch.equal(want, ovc.attention_packed(*arguments))
+    forward.check_status(device)
