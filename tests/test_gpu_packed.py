@@ -403,3 +403,20 @@ def test_rows_without_keys_beside_values_that_are_not_finite(q_lens, k_lens, hq,
     assert bool(blind.any()) and not bool(blind.all())
     assert not out[blind].any() and bool((lse[:, blind] == -math.inf).all())
     assert not bool(torch.isfinite(out[~blind]).any()) and bool(torch.isfinite(lse[:, ~blind]).all())
+
+
+@pytest.mark.parametrize("q_lens,k_lens,hq,hk", [([9, 200], [700, 0], 37, 37), ([130, 200], [300, 9], 7, 1),  # whole
+                                                 ([9, 250], [900, 300], 2, 2), ([3, 20], [900, 200], 7, 1)])  # wide, narrow split
+def test_what_lies_behind_a_sequence_in_its_query_tile(q_lens, k_lens, hq, hk):
+    """The next sequence's queries share a tile with the first one's last rows, and are not finite."""
+    ovc = _ovc()
+    q, k, v = inputs(q_lens, k_lens, hq, hk, torch.float16, 41)
+    cu = cumulative(q_lens), cumulative(k_lens)
+    end = q_lens[0]
+    want, want_lse = ovc.attention_packed(q, k, v, *cu, return_lse=True)
+    close(want[:end], want_lse[:, :end], q[:end], k[:k_lens[0]], v[:k_lens[0]], q_lens[:1], k_lens[:1], False)
+    for bad in (math.nan, math.inf, -math.inf, 0.0):
+        q[end:] = bad
+        out, lse = ovc.attention_packed(q, k, v, *cu, return_lse=True)
+        assert torch.equal(out[:end], want[:end]) and torch.equal(lse[:, :end], want_lse[:, :end])
+    _check_status()
