@@ -237,7 +237,9 @@ int ovc_attention_ex(const void* q8, const void* k8, const void* v_packed, const
  *   y = turn(x * w / sqrt(mean(x^2) + eps)); each pair (a, b) of a head's channels becomes
  *   (a cos t - b sin t, a sin t + b cos t), t = 2 pi * turns[pair] * positions[token][pair_axis[pair]],
  * computed in float32 (t modulo one turn, in 64-bit fixed point) and rounded once.  Pair p is the channels (2p, 2p + 1),
- * or with half_split (p, p + 64); turns[p] = 0 leaves a pair unturned.  A null weight means no norm for that tensor.
+ * or with half_split (p, p + 64); turns[p] = 0 leaves a pair as it is (bit for bit in a 16-bit output without norm).  A null
+ * weight means no norm for that tensor; a normalised head with a value that is not finite has only zeros and NaN, and which
+ * of them are NaN is not defined.
  */
 #define OVC_POSITIONS_I32 0
 #define OVC_POSITIONS_I64 1

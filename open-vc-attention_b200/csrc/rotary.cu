@@ -38,6 +38,7 @@ struct Angles {
     float eps;
     unsigned long long turns[kPairs];  // per position, in units of 2^-64 turns, without the whole turns
     int whole[kPairs];                 // the whole turns, rounded down; 0 unless the positions are float32
+    unsigned long long still;          // bit p: pair p is not turned
     uint8_t axis[kPairs];
 };
 
@@ -180,6 +181,28 @@ __device__ __forceinline__ void turn(Four& v, const Turns& t) {
     }
 }
 
+// Pairs that are not turned keep their values whatever the other member holds: zero times an infinity is NaN, so their members
+// enter each other's products as zero.  `moving` has a bit for each of the lane's pairs that turns.
+__device__ __forceinline__ uint64_t moving_mask(uint32_t moving, int i) {
+    return pack_u2(moving >> 2 * i & 1 ? ~0u : 0u, moving >> 2 * i & 2 ? ~0u : 0u);
+}
+__device__ __forceinline__ void turn_moving(Four& v, const Turns& t, uint32_t moving) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t a = v.a[i], b = v.b[i], mask = moving_mask(moving, i);
+        v.a[i] = ffma2(a, t.c[i], fmul2(b & mask, t.minus_s[i]));
+        v.b[i] = ffma2(a & mask, t.s[i], fmul2(b, t.c[i]));
+    }
+}
+__device__ __forceinline__ void turn_moving(Four& v, const Mix& t, uint32_t moving) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint64_t a = v.a[i], b = v.b[i], mask = moving_mask(moving, i);
+        v.a[i] = ffma2(a, t.aa[i], fmul2(b & mask, t.ab[i]));
+        v.b[i] = ffma2(a & mask, t.ba[i], fmul2(b, t.bb[i]));
+    }
+}
+
 // Sums over the sixteen lanes of a head for N = 2, 4 or 8 heads at once: steps in which a lane gives half of its sums away and
 // adds up the other half, so that 4 sums cost 5 exchanges instead of 16.  Lane lane_of_sum<N>(i) is left with sum i.
 template <int N>
@@ -259,7 +282,10 @@ __device__ __forceinline__ void wait_copies() {
 // power limit leaves after some hundred calls (1.61 GHz): 125 us (805 MB; a copy of that size takes 123 us); with the weights
 // loaded and multiplied head by head 131, and with the unit's place found by a 64-bit division 138.  (Groups of one tensor:
 // heads of either in a row, which cost every head a choice of pointers and weights, took 143 us where this took 122.)
-template <int DT, bool kHalf, bool kNorm>
+// kStill, where the plan has pairs that are not turned and a tensor without norm: such pairs keep their values beside an
+// infinity.  It costs nothing without norm, 10 % (registers) where only one of the tensors has it.  (A normalised head that holds
+// an infinity has nothing but zeros and NaN left.)
+template <int DT, bool kHalf, bool kNorm, bool kStill>
 __global__ void __launch_bounds__(32 * kUnitWarps, 7)
 rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_groups) {
     extern __shared__ __align__(16) uint8_t staged[];
@@ -297,7 +323,11 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_groups) {
         cs[i] = side ? c : t.x, cs[2 + i] = side ? t.x : c;
         sn[i] = side ? s : t.y, sn[2 + i] = side ? t.y : s;
     }
-    const Turns turns = make_turns(make_float4(cs[0], cs[1], cs[2], cs[3]), make_float4(sn[0], sn[1], sn[2], sn[3]));
+    Turns turns = make_turns(make_float4(cs[0], cs[1], cs[2], cs[3]), make_float4(sn[0], sn[1], sn[2], sn[3]));
+    const uint32_t moving = kStill ? ~static_cast<uint32_t>(a.angles.still >> 4 * c16) : 0u;
+    if (kStill)  // zero times minus zero added to either member keeps the sign of a zero
+#pragma unroll
+        for (int i = 0; i < 2; ++i) turns.s[i] |= pack_u2(moving >> 2 * i & 1 ? 0u : 0x80000000u, moving >> 2 * i & 2 ? 0u : 0x80000000u);
 
     Mix mix;
     for (int j = 0; j < count; ++j) {
@@ -340,7 +370,9 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_groups) {
         uint16_t* const y = static_cast<uint16_t*>(t.y) + (token * t.heads + head) * kDim + (kHalf ? 4 : 8) * c16;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            if (kNorm) turn(v[i], mix);
+            if (kNorm && kStill && t.weight == nullptr) turn_moving(v[i], mix, moving);
+            else if (kNorm) turn(v[i], mix);
+            else if (kStill) turn_moving(v[i], turns, moving);
             else turn(v[i], turns);
             float f[8];
             in_order<kHalf>(v[i], f);
@@ -365,10 +397,10 @@ rotary_kernel(const __grid_constant__ RotaryArgs a, int unit_groups) {
 // of a row is not multiplied into its values but into the row's maximum and scale.
 // [73397, 14 + 14, 128]: 146 us, with norm 162 us (789 MB: 120 us at the rate of a copy); with norm it issues on two of three
 // cycles.  Next head in registers: 155 / 185 us.  Max |v| found on the way, instead of by the kernel behind it: 17 us more in
-// all.
+// all.  kStill as above, 1 % and 7 %.
 constexpr int kQuantThreads = 512, kQuantRows = kTile * 16 / kQuantThreads, kQuantStep = kQuantThreads / 16;
 
-template <int DT, bool kHalf, bool kNorm>
+template <int DT, bool kHalf, bool kNorm, bool kStill>
 __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __grid_constant__ RotaryArgs a, int blocks, int rows_per_cta) {
     extern __shared__ __align__(16) float table[];  // cos [128][64], sin [128][64]
     __shared__ uint32_t part[2][kQuantThreads / 32];
@@ -399,6 +431,7 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    const uint32_t moving = kStill ? ~static_cast<uint32_t>(a.angles.still >> 4 * c16) : 0u;
     release_next();  // the kernel behind may read V where this one leaves room
     load(first);
     stage_pairs(a.angles, pairs);
@@ -430,7 +463,9 @@ __global__ void __launch_bounds__(kQuantThreads, 2) rotary_quant_kernel(const __
 #pragma unroll
         for (int i = 0; i < kQuantRows; ++i) {
             const float* from = table + (r0 + kQuantStep * i) * kPairs + 4 * c16;
-            turn(v[i], make_turns(*reinterpret_cast<const float4*>(from), *reinterpret_cast<const float4*>(from + kTile * kPairs)));
+            const Turns turns = make_turns(*reinterpret_cast<const float4*>(from), *reinterpret_cast<const float4*>(from + kTile * kPairs));
+            if (kStill && !norm) turn_moving(v[i], turns, moving);
+            else turn(v[i], turns);
             float f[8];
             in_order<kHalf>(v[i], f);
             float top = fmax3(fabsf(f[0]), fabsf(f[1]), fabsf(f[2]));
@@ -492,6 +527,7 @@ bool take_angles(const ovc_rotary* r, Angles* out) {
             if (!(size < kMostTurns)) return false;
             out->whole[i] = negative ? -static_cast<int>(whole) - (fraction != 0) : static_cast<int>(whole);
         }
+        if (fraction == 0 && out->whole[i] == 0) out->still |= 1ull << i;
         out->axis[i] = r->pair_axis[i];
     }
     return true;
@@ -506,14 +542,18 @@ bool take_source(const void* x, void* y, const float* weight, const int64_t* str
     return true;
 }
 
-// launch(bf16, half, norm) with the three as compile-time constants.
+// launch(bf16, half, norm, still) with the four as compile-time constants.
 template <class Launch>
-int by_variant(int dtype, const ovc_rotary* r, Launch launch) {
-    const auto norm = [&](auto bf16, auto half) {
-        return r->q_weight || r->k_weight ? launch(bf16, half, std::true_type{}) : launch(bf16, half, std::false_type{});
+int by_variant(int dtype, const ovc_rotary* r, const Angles& angles, Launch launch) {
+    const auto by_still = [&](auto bf16, auto half, auto norm) {
+        const bool both = r->q_weight && r->k_weight;
+        return angles.still && !both ? launch(bf16, half, norm, std::true_type{}) : launch(bf16, half, norm, std::false_type{});
     };
-    const auto half = [&](auto bf16) { return r->half_split ? norm(bf16, std::true_type{}) : norm(bf16, std::false_type{}); };
-    return dtype == OVC_BF16 ? half(std::true_type{}) : half(std::false_type{});
+    const auto by_norm = [&](auto bf16, auto half) {
+        return r->q_weight || r->k_weight ? by_still(bf16, half, std::true_type{}) : by_still(bf16, half, std::false_type{});
+    };
+    const auto by_half = [&](auto bf16) { return r->half_split ? by_norm(bf16, std::true_type{}) : by_norm(bf16, std::false_type{}); };
+    return dtype == OVC_BF16 ? by_half(std::true_type{}) : by_half(std::false_type{});
 }
 
 bool bad_shape(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk) {
@@ -526,6 +566,26 @@ bool bad_shape(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk) {
 
 using namespace ovc;
 
+namespace {
+
+int launch_rotary(const RotaryArgs& a, int dtype, const ovc_rotary* rotary, void* stream) {
+    // A unit has up to four groups of eight heads, fewer where that would leave SMs without a few warps each.
+    const int64_t groups = ceil_div(a.src[0].heads, kGroupRows) + ceil_div(a.src[1].heads, kGroupRows), share = a.tokens * groups / (8 * 148);
+    int64_t unit_groups = share > kUnitGroups ? kUnitGroups : share < 1 ? 1 : share;
+    const int64_t units = ceil_div(groups, unit_groups);
+    unit_groups = ceil_div(groups, units);
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, kUnitWarps)), static_cast<unsigned>(units));
+    const size_t smem = static_cast<size_t>(kUnitWarps * unit_groups * kGroupRows * 256);
+    auto s = static_cast<cudaStream_t>(stream);
+    return by_variant(dtype, rotary, a.angles, [&](auto bf16, auto half, auto norm, auto still) {
+        rotary_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value, still.value>
+            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(unit_groups));
+        return check_launch();
+    });
+}
+
+}  // namespace
+
 extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype, int64_t B,
                              int64_t S, int64_t Hq, int64_t Hk, const ovc_rotary* rotary, void* q_out, void* k_out, void* stream) {
     RotaryArgs a{};
@@ -534,20 +594,7 @@ extern "C" int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void
         !take_source(k, k_out, rotary->k_weight, k_strides, Hk, 15, &a.src[1]))
         return OVC_ERR_ARGUMENT;
     a.S = S, a.tokens = B * S;
-    // A unit has up to four groups of eight heads, fewer where that would leave SMs without a few warps each.
-    const int64_t groups = ceil_div(Hq, kGroupRows) + ceil_div(Hk, kGroupRows), share = a.tokens * groups / (8 * 148);
-    int64_t unit_groups = share > kUnitGroups ? kUnitGroups : share < 1 ? 1 : share;
-    const int64_t units = ceil_div(groups, unit_groups);
-    unit_groups = ceil_div(groups, units);
-    const dim3 grid(static_cast<unsigned>(ceil_div(a.tokens, kUnitWarps)), static_cast<unsigned>(units));
-    const size_t smem = static_cast<size_t>(kUnitWarps * unit_groups * kGroupRows * 256);
-    auto s = static_cast<cudaStream_t>(stream);
-    const auto launch = [&](auto bf16, auto half, auto norm) {
-        rotary_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>
-            <<<grid, 32 * kUnitWarps, smem, s>>>(a, static_cast<int>(unit_groups));
-        return check_launch();
-    };
-    return by_variant(dtype, rotary, launch);
+    return launch_rotary(a, dtype, rotary, stream);
 }
 
 namespace {
@@ -576,8 +623,8 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(rows, per_cta)), static_cast<unsigned>(B));
     constexpr int smem = kTile * kPairs * static_cast<int>(sizeof(float2)) + kTile * kDim * 2;
     auto s = static_cast<cudaStream_t>(stream);
-    const auto launch = [&](auto bf16, auto half, auto norm) {
-        const auto kernel = rotary_quant_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value>;
+    const auto launch = [&](auto bf16, auto half, auto norm, auto still) {
+        const auto kernel = rotary_quant_kernel<bf16.value ? OVC_BF16 : OVC_F16, half.value, norm.value, still.value>;
         static std::atomic<unsigned long long> ready;  // devices on which the kernel may take that much
         int device = 0;
         cudaError_t err = cudaGetDevice(&device);
@@ -589,7 +636,7 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
         kernel<<<grid, kQuantThreads, smem, s>>>(a, static_cast<int>(blocks), per_cta);
         return check_launch();
     };
-    return by_variant(dtype, rotary, launch);
+    return by_variant(dtype, rotary, a.angles, launch);
 }
 
 }  // namespace

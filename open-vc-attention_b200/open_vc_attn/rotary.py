@@ -58,7 +58,7 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
                  positions are allowed).  ``grid_positions`` makes those of a clip.  Contiguous ones are referred to and read by
                  every call and replay, so that a captured step may count on in place; others are copied here.
     axes         channels of each of the A axes, in the order of the head's channels: even, 128 in all or fewer; channels
-                 behind them stay as they are (interleaved pairs only).
+                 behind them are not turned (interleaved pairs only): without a norm they stay as they are, whatever they hold.
     theta        pair i of an axis with d channels turns by theta^(-2 i / d) radians per position (below 2^30 turns, where
                  positions are float32).  With ``frequencies="head"`` i and d count over all axes together (sections of one
                  set of frequencies).

@@ -366,3 +366,64 @@ def test_frequencies_of_any_size_and_sign(kind, half):
     d = prepared.k_descale.double()[0, :, 0][None, :, None]
     limit = (want / d).abs().mul(2.0 ** -4).clamp_min(2.0 ** -10) + 1.1 * (F32 * size / d + 4 * 2.0 ** -24 * (want / d).abs())
     assert bool(((prepared.k.double() - want / d).abs() <= limit).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("axes", [(40, 40, 40), (2, 2, 2), (4, 2, 120)])
+@pytest.mark.parametrize("weighted", ["none", "q", "k"])
+def test_channels_without_an_axis_stay_as_they_are(dtype, axes, weighted):
+    """Zeros of either sign, infinities and NaN beside each other: the tensors that are not normalised keep every bit."""
+    ovc = _ovc()
+    s, total = 70, sum(axes)
+    q, k, (qw, kw) = inputs((s, 9, 128), (s, 3, 128), total, dtype)
+    special = torch.tensor([math.inf, 1.5, -0.0, math.nan, 2.0, -math.inf, -0.0, -3.0, 0.0, -0.0], device=DEV, dtype=dtype)
+    rest = 128 - total
+    if rest:
+        pick = torch.randint(0, 10, (s, 3, rest), device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+        q[:, :3, total:], k[..., total:] = special[pick], special[pick.flip(-1)]
+    positions = torch.randint(0, 5000, (s, 3), device=DEV, dtype=torch.int32, generator=torch.Generator(device=DEV).manual_seed(2))
+    plan = ovc.rotary_plan(positions, axes=axes, q_weight=qw if weighted == "q" else None, k_weight=kw if weighted == "k" else None)
+    for name, x, y in zip("qk", (q, k), ovc.rotary_qk(q, k, plan)):
+        if name != weighted:
+            kept = [t[..., total:].contiguous().view(torch.int16) for t in (x, y)]
+            nan = x[..., total:].isnan()
+            assert torch.equal(kept[0][~nan], kept[1][~nan]) and torch.equal(nan, y[..., total:].isnan())
+        finite = torch.isfinite(x).all(-1) if name == weighted else torch.ones(x.shape[:2], dtype=torch.bool, device=DEV)
+        want, size = formula(x, positions, axes, weight=qw if weighted == "q" else kw if weighted == "k" else None) if name == weighted \
+            else formula(x, positions, axes)
+        close(y[finite][..., :total], want[finite][..., :total], size[finite][..., :total])
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_single_pairs_that_do_not_turn(half):
+    """Frequencies of zero anywhere among the pairs, in either layout, at the C entry."""
+    ovc = _ovc()
+    plan = ovc.rotary_plan(torch.arange(50, device=DEV)[:, None], axes=(128,), interleaved=not half)
+    turns = [0.0 if i % 3 == 0 or i in (7, 62) else 2.0 ** -(i % 11) for i in range(64)]
+    plan.turns[:] = turns
+    q, k, _ = inputs((50, 2, 128), (50, 5, 128), 3, torch.bfloat16)
+    still = torch.tensor([i for i, t in enumerate(turns) if t == 0.0], device=DEV)
+    at, to = (still, still + 64) if half else (2 * still, 2 * still + 1)
+    q[:, 0, at], k[:, 1, to] = math.inf, -math.inf
+    for x, y in zip((q, k), ovc.rotary_qk(q, k, plan)):
+        assert torch.equal(x[..., at], y[..., at]) and torch.equal(x[..., to], y[..., to])
+        clean = x.masked_fill(torch.isinf(x), 0.0)
+        want, size = turned(clean, torch.arange(50, device=DEV)[:, None], torch.tensor(turns, device=DEV, dtype=torch.float64), half)
+        moved = torch.tensor([c for c in range(128) if c not in set(at.tolist() + to.tolist())], device=DEV)
+        close(y[..., moved], want[..., moved], size[..., moved])
+
+
+@pytest.mark.parametrize("weighted", [False, True])
+def test_preparation_keeps_channels_without_an_axis(weighted):
+    """A NaN takes no part in its block's scale; the channel beside it, not turned, has the code of its own value."""
+    from open_vc_attn.quantization import fp8_quantize_per_block
+
+    ovc = _ovc()
+    q, k, (qw, _) = inputs((300, 2, 128), (300, 2, 128), 8, torch.bfloat16)
+    plan = ovc.rotary_plan(torch.zeros(300, 3, device=DEV, dtype=torch.int32), axes=(40, 40, 40), q_weight=qw if weighted else None)
+    k[::7, :, 124] = math.nan
+    got = ovc.prepare_fp8(q, k, k, rotary=plan)
+    want, descale = fp8_quantize_per_block(k, block_l=128)
+    keep = [c for c in range(128) if c != 124]
+    assert torch.equal(got.k_descale, descale)
+    assert torch.equal(got.k[..., keep].view(torch.uint8), want[0][..., keep].view(torch.uint8))  # (the quantiser's output is batched)
