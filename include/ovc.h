@@ -272,6 +272,8 @@ int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const 
  * rotated values are not rounded to 16 bits in between.
  *   q, k, v dense [B,S,H,128]; q8, k8, v8 the same in fp8; q_descale, k_descale [B,H,ceil(S/128)], v_descale [B,H];
  *   amax_ws [B,H] f32 scratch (holds the per-head max |v| afterwards).
+ *   A NaN takes no part in a scale and has the code of NaN (ovc_quantize_per_block: that of -448); so has an infinity, whose
+ *   block has scale infinity and otherwise zeros.
  *   cu_seqlens [2] int32 or NULL, B == 1 only: set to 0 and S, for callers that hand such bounds on.
  */
 int ovc_prepare_rotary(const void* q, const void* k, const void* v, int dtype, int64_t B, int64_t S, int64_t H,

@@ -427,3 +427,49 @@ def test_preparation_keeps_channels_without_an_axis(weighted):
     keep = [c for c in range(128) if c != 124]
     assert torch.equal(got.k_descale, descale)
     assert torch.equal(got.k[..., keep].view(torch.uint8), want[0][..., keep].view(torch.uint8))  # (the quantiser's output is batched)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("axes,interleaved", [((44, 42, 42), True), ((128,), False), ((40, 40, 40), True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_codes_of_values_that_are_not_finite(bad, axes, interleaved, dtype):
+    """At position zero a rotation without norm leaves 16-bit values that rotary_qk rounds to themselves (and NaN, where zero
+    times an infinity is added), so the preparation has the codes and scales of the quantiser on rotary_qk's output, but NaN
+    for what is not finite, where that has -448."""
+    from open_vc_attn.quantization import fp8_quantize_per_block
+
+    ovc = _ovc()
+    q, k, _ = inputs((700, 2, 128), (700, 2, 128), 19, dtype)
+    q[130, 1, 3], q[131, :, 127], q[5, 0, 64] = bad, bad, bad
+    k[300:400], k[699, 1, 121] = bad, bad
+    plan = ovc.rotary_plan(torch.zeros(700, len(axes), device=DEV, dtype=torch.int32), axes=axes, interleaved=interleaved)
+    got = ovc.prepare_fp8(q, k, k, rotary=plan)
+    for x, codes, descale in zip(ovc.rotary_qk(q, k, plan), (got.q, got.k), (got.q_descale, got.k_descale)):
+        want, want_descale = fp8_quantize_per_block(x, block_l=128)
+        assert torch.equal(descale, want_descale)
+        odd = ~torch.isfinite(x)
+        assert bool(odd.any()) and bool((want[0].float()[odd].abs() == 448).all())
+        assert bool(codes.float()[odd].isnan().all()) and torch.equal(codes.view(torch.uint8)[~odd], want[0].view(torch.uint8)[~odd])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_codes_of_normalised_heads_that_are_not_finite(bad):
+    """Such a head has NaN (an infinity over an infinity) and zeros; other heads keep their codes, the block its scale."""
+    ovc = _ovc()
+    q, k, (qw, kw) = inputs((200, 3, 128), (200, 3, 128), 20, torch.bfloat16)
+    positions = torch.arange(200, device=DEV)[:, None]
+    plan = ovc.rotary_plan(positions, axes=(128,), q_weight=qw, k_weight=kw)
+    q[7, 1] = 0.0
+    clean = ovc.prepare_fp8(q, k, k, rotary=plan)
+    q[7, 1, 10] = bad
+    got = ovc.prepare_fp8(q, k, k, rotary=plan)
+    codes, was = got.q.view(torch.uint8), clean.q.view(torch.uint8)
+    assert torch.equal(got.q_descale, clean.q_descale) and torch.equal(got.k.view(torch.uint8), clean.k.view(torch.uint8))
+    rotated = ovc.rotary_qk(q, k, plan)[0]
+    nan = rotated.isnan()
+    assert bool(nan[7, 1, 10]) and int(nan.any(-1).sum()) == 1
+    assert torch.equal(got.q.float().isnan(), nan)
+    others = torch.ones(200, 3, dtype=torch.bool, device=DEV)
+    others[7, 1] = False
+    assert torch.equal(codes[others], was[others])
+    assert bool((codes[7, 1][~nan[7, 1]] & 0x7F == 0).all())
