@@ -263,6 +263,7 @@ typedef struct ovc_rotary {
  * Rotated (and normalised) Q and K in their own 16-bit type.
  *   q [B,S,Hq,128], k [B,S,Hk,128]: strides[3] = elements from one batch item, token and head to the next, multiples
  *   of 8 (a slice of a fused projection is read in place); q_out, k_out dense, not overlapping q or k.
+ *   B * S < 2^31, S <= 2^30; Hq, Hk <= 65535.
  */
 int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype, int64_t B,
                   int64_t S, int64_t Hq, int64_t Hk, const ovc_rotary* rotary, void* q_out, void* k_out, void* stream);
@@ -272,6 +273,7 @@ int ovc_rotary_qk(const void* q, const int64_t* q_strides, const void* k, const 
  * rotated values are not rounded to 16 bits in between.
  *   q, k, v dense [B,S,H,128]; q8, k8, v8 the same in fp8; q_descale, k_descale [B,H,ceil(S/128)], v_descale [B,H];
  *   amax_ws [B,H] f32 scratch (holds the per-head max |v| afterwards).
+ *   B <= 32767; H <= 65535.
  *   A NaN takes no part in a scale and has the code of NaN (ovc_quantize_per_block: that of -448); so has an infinity, whose
  *   block has scale infinity and otherwise zeros.
  *   cu_seqlens [2] int32 or NULL, B == 1 only: set to 0 and S, for callers that hand such bounds on.

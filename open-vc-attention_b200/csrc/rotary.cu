@@ -557,8 +557,8 @@ int by_variant(int dtype, const ovc_rotary* r, const Angles& angles, Launch laun
 }
 
 bool bad_shape(int dtype, int64_t B, int64_t S, int64_t Hq, int64_t Hk) {
-    return (dtype != OVC_F16 && dtype != OVC_BF16) || B < 1 || S < 1 || Hq < 1 || Hk < 1 || Hq > 65535 || Hk > 65535 || B > 32767 ||
-           S > (1LL << 30) || B * S > 0x7FFFFFFFLL;
+    return (dtype != OVC_F16 && dtype != OVC_BF16) || B < 1 || S < 1 || Hq < 1 || Hk < 1 || Hq > 65535 || Hk > 65535 ||
+           B > 0x7FFFFFFFLL || S > (1LL << 30) || B * S > 0x7FFFFFFFLL;
 }
 
 }  // namespace
@@ -605,7 +605,7 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     const int64_t blocks = ceil_div(S, kTile);
     const int64_t strides[3] = {S * H * kDim, H * kDim, kDim};
     RotaryArgs a{};
-    if (bad_shape(dtype, B, S, H, H) || !q_descale || !k_descale || q_stride < blocks || k_stride < blocks || !take_angles(rotary, &a.angles) ||
+    if (bad_shape(dtype, B, S, H, H) || B > 32767 || !q_descale || !k_descale || q_stride < blocks || k_stride < blocks || !take_angles(rotary, &a.angles) ||
         !take_source(q, q8, rotary->q_weight, strides, H, 7, &a.src[0]) || !take_source(k, k8, rotary->k_weight, strides, H, 7, &a.src[1]))
         return OVC_ERR_ARGUMENT;
     a.S = S, a.tokens = B * S, a.amax_init = amax_init, a.bounds = bounds;
@@ -614,11 +614,12 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     // Two CTAs run per SM.  Heads per CTA: the count whose rounds of CTAs, each of its heads and the block's angles (which
     // cost about as much as two heads), are the shortest in all.
     const int rows = static_cast<int>(2 * H);
-    int per_cta = 1;
+    const int least = rows > 65535 ? 2 : 1;  // (the grid's second index)
+    int per_cta = least;
     int64_t best = 0;
-    for (int n = 1; n <= rows; ++n) {
+    for (int n = least; n <= rows; ++n) {
         const int64_t cost = ceil_div(blocks * B * ceil_div(rows, n), 2 * 148) * (n + 2);
-        if (n == 1 || cost <= best) best = cost, per_cta = n;
+        if (n == least || cost <= best) best = cost, per_cta = n;
     }
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(rows, per_cta)), static_cast<unsigned>(B));
     constexpr int smem = kTile * kPairs * static_cast<int>(sizeof(float2)) + kTile * kDim * 2;

@@ -473,3 +473,24 @@ def test_codes_of_normalised_heads_that_are_not_finite(bad):
     others[7, 1] = False
     assert torch.equal(codes[others], was[others])
     assert bool((codes[7, 1][~nan[7, 1]] & 0x7F == 0).all())
+
+
+@pytest.mark.parametrize("per_item", [False, True])
+def test_a_batch_of_many_short_sequences(per_item):
+    """More items than the grid's third index counts: rotary_qk has no use for it."""
+    ovc = _ovc()
+    q, k, _ = inputs((70001, 3, 1, 128), (70001, 3, 2, 128), 23, torch.bfloat16)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    positions = torch.randint(0, 3000, (70001, 3, 1) if per_item else (3, 1), generator=g, device=DEV)
+    for x, y in zip((q, k), ovc.rotary_qk(q, k, ovc.rotary_plan(positions, axes=(128,)))):
+        close(y, *formula(x, positions, (128,)))
+
+
+def test_preparation_of_more_heads_than_a_grid_counts():
+    ovc = _ovc()
+    q, k, _ = inputs((1, 40000, 128), (1, 40000, 128), 24, torch.bfloat16)
+    plan = ovc.rotary_plan(torch.full((1, 1), 7, device=DEV), axes=(128,))
+    got, few = ovc.prepare_fp8(q, k, k, rotary=plan), ovc.prepare_fp8(q[:, -3:], k[:, -3:], k[:, -3:], rotary=plan)
+    for a, b in zip((got.q, got.k, got.v), (few.q, few.k, few.v)):
+        assert torch.equal(a[:, -3:].view(torch.uint8), b.view(torch.uint8))
+    assert torch.equal(got.q_descale[:, -3:], few.q_descale) and torch.equal(got.k_descale[:, -3:], few.k_descale)
