@@ -16,6 +16,7 @@ import torch
 from . import _lib
 
 _Three = ctypes.c_int64 * 3
+_LARGEST_EPS = torch.finfo(torch.float32).max
 _MOST_TURNS = 2.0 ** 30  # per float32 position: the kernels carry the whole turns in 32 bits
 _POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 
@@ -82,8 +83,8 @@ def rotary_plan(positions, *, axes=(44, 42, 42), theta=10000.0, interleaved=True
         raise ValueError("frequencies must be axis or head")
     if not (math.isfinite(theta) and theta > 0.0):
         raise ValueError("theta must be positive and finite")
-    if not (math.isfinite(eps) and eps >= 0.0):
-        raise ValueError("eps must be finite and not negative")
+    if not 0.0 <= eps <= _LARGEST_EPS:
+        raise ValueError("eps must be finite, in float32 as well, and not negative")
     if not positions.is_cuda:
         raise ValueError("positions must reside on a CUDA device")
     if positions.requires_grad:

@@ -136,3 +136,9 @@ def _float_plan_on_meta(**options):
         is_cuda = True
 
     return open_vc_attn.rotary_plan(torch.zeros(4, 1).as_subclass(Positions), axes=(128,), **options)
+
+
+@pytest.mark.parametrize("eps", [1e39, float("inf"), -1e-30])
+def test_plan_refuses_an_eps_that_float32_cannot_hold(eps):
+    with pytest.raises(ValueError, match="eps"):
+        _float_plan_on_meta(eps=eps)
