@@ -614,12 +614,12 @@ int launch_rotary_quant(const void* q, const void* k, int dtype, int64_t B, int6
     // Two CTAs run per SM.  Heads per CTA: the count whose rounds of CTAs, each of its heads and the block's angles (which
     // cost about as much as two heads), are the shortest in all.
     const int rows = static_cast<int>(2 * H);
-    const int least = rows > 65535 ? 2 : 1;  // (the grid's second index)
-    int per_cta = least;
+    // (With hundreds of heads the angles are shared by many, so the grid's second index stays far below its limit.)
+    int per_cta = 1;
     int64_t best = 0;
-    for (int n = least; n <= rows; ++n) {
+    for (int n = 1; n <= rows; ++n) {
         const int64_t cost = ceil_div(blocks * B * ceil_div(rows, n), 2 * 148) * (n + 2);
-        if (n == least || cost <= best) best = cost, per_cta = n;
+        if (n == 1 || cost <= best) best = cost, per_cta = n;
     }
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(rows, per_cta)), static_cast<unsigned>(B));
     constexpr int smem = kTile * kPairs * static_cast<int>(sizeof(float2)) + kTile * kDim * 2;
