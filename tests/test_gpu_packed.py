@@ -420,3 +420,46 @@ def test_what_lies_behind_a_sequence_in_its_query_tile(q_lens, k_lens, hq, hk):
         out, lse = ovc.attention_packed(q, k, v, *cu, return_lse=True)
         assert torch.equal(out[:end], want[:end]) and torch.equal(lse[:, :end], want_lse[:, :end])
     _check_status()
+
+
+LYING = [[0, 100, 2 ** 31 - 1], [0, 100, -5], [0, -(2 ** 31), 300], [0, 300, 0, 300, 0, 300, 0, 300, 0, 300], [250, 20, 290, 7],
+         [2 ** 31 - 1, -(2 ** 31), 2 ** 31 - 1], [-7, 3, 3, 299, 301, 300]]
+
+
+@pytest.mark.parametrize("tq,tk,hq,hk", [(300, 300, 80, 80), (300, 200, 7, 1),  # whole
+                                         (300, 3000, 4, 2), (300, 3000, 3, 3),  # wide split
+                                         (30, 6000, 4, 1), (18, 3000, 9, 9)])  # narrow split
+@pytest.mark.parametrize("causal", [False, True])
+def test_bounds_that_lie_write_nothing_beside_the_outputs(tq, tk, hq, hk, causal):
+    """Through the C entry: output, log-sum-exp and workspace are pieces of larger tensors whose other elements keep their
+    values.  (That no access leaves them is shown by the clamps of bounds() and of the plan; this finds a mistake in them.)"""
+    from ctypes import c_int64
+
+    from open_vc_attn import _lib
+    from open_vc_attn.forward import _status
+
+    lib = _lib.load()
+    q, k, v = inputs([tq], [tk], hq, hk, torch.bfloat16, 8)
+    words, mirror = _status(torch.device(DEV))
+    strides = [(c_int64 * 2)(h * 128, 128) for h in (hq, hk)]
+    pad = 1024  # rows, elements
+    for shape in LYING:
+        cu = [torch.tensor([max(-(2 ** 31), min(2 ** 31 - 1, x * n // 300)) for x in shape], dtype=torch.int32, device=DEV) for n in (tq, tk)]
+        sizes = (len(shape) - 1, tq, tk, hq, hk)
+        out = torch.full((pad + tq + pad, hq, 128), 7.0, device=DEV, dtype=q.dtype)
+        lse = torch.full((pad + hq * tq + pad,), 7.0, device=DEV)
+        size = lib.ovc_attention_packed_workspace(*sizes)
+        assert size % 4 == 0
+        work = torch.full((pad + size // 4 + pad,), 7.0, device=DEV)
+        for flags in (0, _lib.OVC_ATTN_ZERO_TAIL):
+            _lib.check(
+                lib.ovc_attention_packed(
+                    q.data_ptr(), strides[0], k.data_ptr(), strides[1], v.data_ptr(), strides[1], _lib.OVC_BF16, cu[0].data_ptr(), cu[1].data_ptr(),
+                    *sizes, flags | (_lib.OVC_ATTN_CAUSAL if causal else 0), 0.1, out[pad:].data_ptr(), lse[pad:].data_ptr(), work[pad:].data_ptr(),
+                    words.data_ptr() + 4, mirror.data_ptr(), torch.cuda.current_stream().cuda_stream,
+                ),
+                "ovc_attention_packed",
+            )
+        _check_status()
+        for t, n in ((out, tq), (lse, hq * tq), (work, size // 4)):
+            assert bool((t[:pad] == 7.0).all()) and bool((t[pad + n:] == 7.0).all())

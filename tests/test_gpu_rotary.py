@@ -494,3 +494,32 @@ def test_preparation_of_more_heads_than_a_grid_counts():
     for a, b in zip((got.q, got.k, got.v), (few.q, few.k, few.v)):
         assert torch.equal(a[:, -3:].view(torch.uint8), b.view(torch.uint8))
     assert torch.equal(got.q_descale[:, -3:], few.q_descale) and torch.equal(got.k_descale[:, -3:], few.k_descale)
+
+
+@pytest.mark.parametrize("batch,s,h", [(1, 300, 2), (3, 129, 2), (2, 500, 3)])
+@pytest.mark.parametrize("kind", ["int32", "int64", "float32"])
+@pytest.mark.parametrize("per_item", [False, True])
+@pytest.mark.parametrize("interleaved,axes,norm", [(True, (44, 42, 42), True), (False, (128,), False)])
+def test_preparation_takes_every_kind_of_positions(batch, s, h, kind, per_item, interleaved, axes, norm):
+    """Tolerances as in test_preparation_rotates_what_it_quantises."""
+    ovc = _ovc()
+    q, k, (qw, kw) = inputs((batch, s, h, 128), (batch, s, h, 128), 31 + s, torch.bfloat16)
+    positions = torch.randint(-3000, 200000, (batch, s, len(axes)) if per_item else (s, len(axes)), device=DEV,
+                              generator=torch.Generator(device=DEV).manual_seed(6))
+    positions = positions.float() / 7.0 if kind == "float32" else positions.to(getattr(torch, kind))
+    plan = ovc.rotary_plan(positions, axes=axes, interleaved=interleaved, q_weight=qw if norm else None, k_weight=kw if norm else None)
+    got = ovc.prepare_fp8(q, k, k, rotary=plan)
+    blocks = -(-s // 128)
+    for x, w, codes, descale in ((q, qw, got.q, got.q_descale), (k, kw, got.k, got.k_descale)):
+        want, size = formula(x, positions, axes, interleaved, weight=w if norm else None)
+        longest, top = [torch.nn.functional.pad(t, (0, 0, 0, 0, 0, blocks * 128 - s)).view(batch, blocks, 128, h, 128).amax((2, 4)).transpose(1, 2)
+                        for t in (size, want.abs())]
+        d = descale.double()
+        assert bool(((d * 448 - top).abs() <= F32 * longest + 4 * 2.0 ** -24 * top).all())
+        per_token = d.transpose(1, 2).repeat_interleave(128, 1)[:, :s, :, None]
+        value, off = want / per_token, F32 * size / per_token + 4 * 2.0 ** -24 * (want / per_token).abs()
+        limit = (value.abs() * 2.0 ** -4).clamp_min(2.0 ** -10) + 1.1 * off
+        assert bool(((codes.double().view(batch, s, h, 128) - value).abs() <= limit).all())
+    if not per_item and batch > 1:  # an item by itself
+        one = ovc.prepare_fp8(q[1], k[1], k[1], rotary=plan)
+        assert torch.equal(one.q.view(torch.uint8), got.q[1].view(torch.uint8)) and torch.equal(one.k_descale[0], got.k_descale[1])
