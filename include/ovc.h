@@ -49,7 +49,7 @@ extern "C" {
 
 #define OVC_STATUS_WAIT_EXPIRED 1u /* a bounded barrier wait gave up; the output rows of that launch hold NaN */
 
-int ovc_version(void);
+int ovc_version(void); /* 2: with ovc_rotary_qk, ovc_prepare_*rotary and ovc_attention_packed* */
 const char* ovc_error_string(int code);
 int ovc_last_cuda_error(void);
 

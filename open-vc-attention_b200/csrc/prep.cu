@@ -422,7 +422,7 @@ int launch_amax_cast_v(const void* v, int dtype, int64_t B, int64_t S, int64_t H
 
 extern "C" {
 
-int ovc_version(void) { return 1; }
+int ovc_version(void) { return 2; }
 
 const char* ovc_error_string(int code) {
     switch (code) {

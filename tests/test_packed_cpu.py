@@ -55,3 +55,10 @@ def test_workspace_sizes():
     assert size(0, 1, 1, 1, 1) == size(1, 1, 1, 3, 2) == size(1, 0, 4096, 1, 1) == 0
     for b, tq, tk, hq, hk in ((16, 16, 200000, 32, 8), (4, 893, 59497, 28, 4), (1, 1, 1 << 30, 128, 1)):
         assert 0 < size(b, tq, tk, hq, hk) < 1 << 30
+
+
+def test_the_version_counts_these_entries():
+    import __graft_entry__
+
+    __graft_entry__.build()
+    assert _lib.load().ovc_version() >= 2
