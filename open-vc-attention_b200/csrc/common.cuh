@@ -24,7 +24,8 @@ inline int check_launch() {
 // A kernel launched behind another of its stream without the gap between them: its CTAs may start as soon as all CTAs of the
 // one before have called release_next() (or have ended) and leave room.  Until wait_for_previous() it may only read what
 // neither of the two writes, and write nothing.  In a kernel launched in the ordinary way both are empty.
-// A preparation with rotation, [32768, 8, 128]: 99 -> 91 us, [1024, 2, 128]: 36 -> 34, [73397, 14, 128]: 281 -> 278.
+// A preparation with rotation and norm in a graph, [32768, 8, 128]: 86 -> 79 us, [1024, 2, 128]: 14.2 -> 12.1,
+// [73397, 14, 128]: 0 to 4 % from run to run; without rotation [32768, 8, 128] 86 -> 82, [73397, 56, 128] 1054 -> 1048.
 template <class... Parameters, class... Arguments>
 int launch_behind(void (*kernel)(Parameters...), dim3 grid, unsigned threads, cudaStream_t stream, Arguments... arguments) {
     cudaLaunchAttribute early{};

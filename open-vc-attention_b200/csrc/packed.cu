@@ -27,13 +27,14 @@
 // What bounds it.  Whole: a step (both stages, one key tile) is 2048 cycles of tensor pipe and as many of exponentials (128 x
 // 128 x 2 at 16 a cycle); it takes about 3300.  A stage's step is a chain - scores read and their maximum found (350 cycles),
 // two halves of exponentials (512 each and what the other stage takes of the unit), P V, Q K^T of the next tile (1120), a
-// few hand-overs of 100 to 200 - and the two stages' chains interleave.  [32768, 8, 128]: 3.6 ms in a row (1.2 PFLOP/s at the
-// power limit, where the library's matrix product reaches 1.4), 3.3 ms alone.  Tried on it, each right and slower: a warp
+// few hand-overs of 100 to 200 - and the two stages' chains interleave.  [32768, 8, 128]: 3.74 ms in a row (1.18 PFLOP/s at the
+// power limit, where the library's matrix product reaches 1.4), 3.34 ms alone.  Tried on it, each right and slower: a warp
 // for the products of each stage (they drift into step: 1.25 times the time), two threads to a row (1.13), part of the
 // exponentials as polynomials on the FMA pipe (1.05 for an eighth to 1.3 for half: a pair costs 25 cycles of issue there and
 // 16 on the special-function unit), the exponentials started with the maximum of the tile before (1.04), a relay that
 // tells the issuing warp of landed tiles (1.03), CTAs that stay and take one row tile after another (1.03).
 // Split, narrow: the rate at which keys are read; 81 us of kernel for 487 MB (6.0 TB/s), 7.2 TB/s once under way.
+// The split forms spill 11 registers of the launch's 168 (44 bytes stored, 64 loaded), the whole form none.
 
 #include <atomic>
 
@@ -969,8 +970,9 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     p.B = static_cast<int>(B), p.Hq = static_cast<int>(Hq), p.Hk = static_cast<int>(Hk), p.G = static_cast<int>(G);
     p.tokens = l.tokens, p.Tq = static_cast<int>(Tq), p.Tk = static_cast<int>(Tk);
     // Narrow: a segment's beginning and end take as long as about four key tiles (with 0, 2, 4, 6 of them sixteen requests
-    // of 129 to 32768 keys took 109, 100, 93, 93 us).  Wide: a key tile takes three times as long, and is cheaper where only
-    // one stage has rows; shares by key tiles alone were the best (0: 218 us, 2: 223, 4: 233 for chunks behind prefixes).
+    // of 129 to 32768 keys took 116, 104, 96, 97 us).  Wide: a key tile takes three times as long, and is cheaper where only
+    // one stage has rows; no count was better than shares by key tiles alone by more than runs differ (0, 2 and 4: 212 to 233
+    // us in changing order for chunks behind prefixes).
     p.segment_cost = l.mode == kSplitNarrow ? 4 : 0;
     p.ctas = static_cast<int>(kSms), p.max_tiles = static_cast<int>(l.tiles < kMaxTiles ? l.tiles : kMaxTiles), p.slot_rows = l.slot_rows;
     p.zero_tail = (flags & OVC_ATTN_ZERO_TAIL) != 0;
@@ -980,9 +982,9 @@ extern "C" int ovc_attention_packed(const void* q, const int64_t* q_strides, con
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     auto s = static_cast<cudaStream_t>(stream);
     // CTAs start in the order of the grid.  Row tile by row tile, with all key heads of each, the long ones of a causal launch
-    // come before the short ones whatever their head (345 -> 334 us for prompts of 5000 to 1 tokens); but the keys and values
+    // come before the short ones whatever their head (356 -> 334 us for prompts of 5000 to 1 tokens); but the keys and values
     // of all heads are in use at once, and where those do not stay in L2 head by head is better (32768 keys of 8 heads, 134 MB:
-    // 3.60 against 3.75 ms).  Half of L2 is the border.
+    // 3.74 against 3.83 ms; two clips of 24 heads, 134 MB as well: 0.89 against 0.91).  Half of L2 is the border.
     p.heads_first = l.mode == kWhole && Tk * Hk * 4 * kDim <= 63LL << 20 && l.tiles <= 65535;
     const dim3 grid = l.mode != kWhole ? dim3(static_cast<unsigned>(kSms))
                       : p.heads_first  ? dim3(static_cast<unsigned>(Hk), static_cast<unsigned>(l.tiles))
