@@ -429,9 +429,11 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         const Shares shares(sm.plan, p);
         at = first_at = shares.first(blockIdx.x), end = shares.first(blockIdx.x + 1);
     }
-    // The next segment, for the whole CTA: false behind the last.  All products and copies of the one before are done.
+    // The next segment, for the whole CTA: false behind the last.  All products and copies of the one before are done, and what
+    // the softmax warps read of its accumulators comes before the next one's products.
     const auto next_segment = [&]() {
         if (at >= end) return false;
+        if (kSplit) tc_fence_before();
         __syncwarp();
         asm volatile("bar.sync 0;" ::: "memory");
         if (warp == 0) {
@@ -453,6 +455,7 @@ packed_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant_
         fence_proxy_async_smem();
         __syncwarp();
         asm volatile("bar.sync 0;" ::: "memory");
+        if (kSplit) tc_fence_after();
         at += kSplit ? item.units : 1;
         return item.valid != 0;
     };

@@ -143,6 +143,7 @@ def test_a_failure_found_in_a_capture_is_reported_again_behind_it():
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
+        arguments[0].neg()  # (so that the graph is not empty)
         with pytest.raises(RuntimeError, match="bounded wait expired"):
             ovc.attention_packed(*arguments)
     with pytest.raises(RuntimeError, match="bounded wait expired"):
